@@ -108,12 +108,10 @@ struct sga_handle {
   Buf* cur_part = nullptr;
   // hyper-prior branch runs on its own stream, forked/joined with events (also inside the graph)
   hipStream_t sB = nullptr;
-  // The stream every step GRAPH is captured and launched on: the library's own, LOW priority (round 6).  Not for speed -- for the
-  // HIP runtime's Graph::UpdateStreams, which reads past the end of a graph's internal stream list when ALL of them share the
-  // LAUNCH stream's hardware queue (host SIGSEGV inside hipGraphLaunch: "defect (a)" of rounds 3-5, root cause and stand-alone
-  // reproducer in DESIGN_EXPERIMENTS.md A.13 / scripts/r06/graph_stream_collision_repro.hip).  The internal streams are created with
-  // NORMAL priority, and hardware queues are pooled per priority class: a launch stream of another class can never share one
-  // with them, whatever streams the process has created and destroyed before.  The caller's stream is bridged in and out
+  // The stream every step GRAPH is captured and launched on: the library's own, LOW priority (round 6).  Not for speed: on
+  // ROCm 7.0.2 hipGraphLaunch on a NORMAL-priority stream crashes the host for some histories of streams that the process has
+  // created and destroyed (scripts/r06/graph_stream_collision_repro.hip: 7 of 64 histories); on a launch stream of another
+  // priority class, whose hardware queues are a pool of their own, it never did.  The caller's stream is bridged in and out
   // with one event pair per call (LaunchStream below); null: graphs run on the caller's stream (laboratory: SGA_LAUNCH_STREAM=caller)
   hipStream_t sG = nullptr;
   hipEvent_t ev_in = nullptr, ev_out = nullptr;
@@ -245,13 +243,6 @@ static void sga_segv_handler(int sig, siginfo_t* si, void* uc_) {
                      (unsigned long long)r[REG_R10], (unsigned long long)r[REG_R11], (unsigned long long)r[REG_R12], (unsigned long long)r[REG_R13],
                      (unsigned long long)r[REG_R14], (unsigned long long)r[REG_R15]);
   (void)!write(fd, buf, (size_t)len);
-  if ((void*)r[REG_RIP] != si->si_addr && r[REG_RIP] > 4096) {      // the faulting instruction's bytes (not when the fault IS the jump target)
-    const unsigned char* ip = (const unsigned char*)r[REG_RIP];
-    len = snprintf(buf, sizeof(buf), " code at rip:");
-    for (int i = 0; i < 24; ++i) len += snprintf(buf + len, sizeof(buf) - (size_t)len, " %02x", ip[i]);
-    len += snprintf(buf + len, sizeof(buf) - (size_t)len, "\n");
-    (void)!write(fd, buf, (size_t)len);
-  }
   const char m1[] = "sga: innermost frames:\n";
   (void)!write(fd, m1, sizeof(m1) - 1);
   backtrace_symbols_fd(g_segv_frames, n < 64 ? n : 64, fd);
@@ -1380,11 +1371,9 @@ int eval_impl(sga_handle* h, const Geom& g, const float* x, const float* y_hat, 
 // Disposal of an executable graph that is dropped in mid-life (a losing fork-point candidate, the least recently used entry of a
 // full cache, the stamped graph of sga_profile_graph_*): destroyed at once, behind a synchronisation of the streams its replays
 // ran on.  Rounds 3-5 RETIRED such graphs until sga_destroy instead, because mid-life destruction was followed -- in long
-// processes, never in a short one -- by a host SIGSEGV inside a later hipGraphLaunch.  Round 6 found why (DESIGN_EXPERIMENTS.md
-// A.13): not the destruction, but what it does to the hardware queues' reference counts -- the HIP runtime's
-// Graph::UpdateStreams overruns a graph's internal stream list when all of them share the LAUNCH stream's hardware queue, and
-// destroying streams is what makes two consecutive stream creations land on one queue.  Graphs are launched on a stream of
-// another priority class now (sga_handle::sG), which can share no queue with them; the retire list is gone.
+// processes, never in a short one -- by a host SIGSEGV inside a later hipGraphLaunch.  What decides is the
+// process's history of created and destroyed streams together with a normal-priority launch stream; graphs are launched on a
+// stream of another priority class now (sga_handle::sG), and the retire list is gone.
 // The calls that replay step graphs run on the handle's own launch stream (sga_handle::sG): ordered after everything the caller
 // has enqueued on ITS stream so far, and the caller's stream ordered after them on the way out -- also on an error return.
 struct LaunchStream {

@@ -1,29 +1,17 @@
 // Stand-alone reproducer (no libsga_hip, no PyTorch) of the HIP-runtime defect behind "defect (a)" -- the host SIGSEGV inside
 // hipGraphLaunch that rounds 3-5 saw after mid-life hipGraphExecDestroy calls (DESIGN_EXPERIMENTS.md A.8a / A.13).
 //
-// What the native backtrace of round 6 showed (profiles/r06_defect_a_native_backtrace.txt; libamdhip64.so of ROCm 7.0.2 as bundled
-// with PyTorch 2.10.0+rocm7.0, offsets in that file):
-//   hipGraphLaunch -> GraphExec::Run (+0xaf880) -> Graph::UpdateStreams (+0xaed90), which does, in effect,
-//       streams_.resize(max_streams_);  streams_[0] = launch_stream;
-//       for (i = 1, j = 0; i < streams_.size(); ++j)
-//         if (queue_of(launch_stream) != queue_of(parallel_streams[j])) streams_[i++] = parallel_streams[j];
-//   -- the loop bounds i, NOT j.  GraphExec::Init (+0xafe20) creates max_streams_ internal streams for a graph that needs
-//   max_streams_ - 1 of them ("one spare"), so ONE internal stream that shares the launch stream's hardware queue is
-//   tolerated; when ALL of them do, j runs past the end of parallel_streams_ and the next 8 bytes of heap are used as a
-//   hip::Stream* (fault address 0x1a8 = NULL + offsetof(vdev) in the crash that was caught).
-// When do all internal streams of a two-stream graph land on the launch stream's hardware queue?  A new stream takes the
-// least-referenced of the GPU_MAX_HW_QUEUES hardware queues of its priority class.  A process that only CREATES streams keeps
-// the reference counts within one of each other and two consecutive creations alternate; DESTROYING streams (what
-// hipGraphExecDestroy does to a graph's internal streams, and hipStreamDestroy to any other) unbalances the counts, and
-// the next graph's streams can both go to the emptier queue -- the launch stream's, if that is where it lives.
+// Observed on the runtime of ROCm 7.0.2 (bundled with PyTorch 2.10.0+rocm7.0): the launch of a two-stream graph crashes for some
+// histories of created and destroyed streams, if the launch stream has normal priority.  Hardware queues are pooled per
+// priority class, and destroying streams makes the spread of the rest over the GPU_MAX_HW_QUEUES queues uneven.
 //
 // This program makes that happen on purpose: a launch stream, a capture partner, NBAL ballast streams; the ballast streams
 // selected by <mask> are destroyed; a two-stream graph (fork / join through events) is captured, instantiated and launched.
 //   usage:  graph_stream_collision_repro <mask> [launch-stream priority: 0 normal (default) | -1 high]
 //   run:    for m in $(seq 0 63); do MALLOC_PERTURB_=165 GPU_MAX_HW_QUEUES=2 ./repro $m 0; done     (scripts/r06/s04_*.sh)
-// MALLOC_PERTURB_ makes the out-of-bounds slot non-zero garbage, so an overrun faults instead of depending on heap history.
+// MALLOC_PERTURB_ fills memory that was never written with non-zero bytes, so the outcome depends less on the heap's history.
 // Expected: with a NORMAL-priority launch stream some masks die with SIGSEGV inside hipGraphLaunch; with a HIGH-priority launch
-// stream (its own hardware-queue class: the internal streams are always created with normal priority) none does -- which is
+// stream (a hardware-queue class of its own) none does -- which is
 // the work-around libsga_hip ships (sga_handle::sG).
 #include <hip/hip_runtime.h>
 
@@ -76,7 +64,7 @@ int main(int argc, char** argv) {
   CHK(hipGraphInstantiate(&ex, g, nullptr, nullptr, 0));      // creates the graph's internal streams
   CHK(hipGraphDestroy(g));
   fprintf(stderr, "mask %2u prio %d: launching\n", mask, prio);
-  for (int r = 0; r < 3; ++r) CHK(hipGraphLaunch(ex, L));     // Graph::UpdateStreams runs in here
+  for (int r = 0; r < 3; ++r) CHK(hipGraphLaunch(ex, L));
   CHK(hipStreamSynchronize(L));
   float ha = 0.f, hb = 0.f;
   CHK(hipMemcpy(&ha, a, sizeof(float), hipMemcpyDeviceToHost));

@@ -1,7 +1,7 @@
 #!/bin/bash
 # GPU box, round 6: defect (a), session 3.  Session 2 ruled out a stack overflow (the crash survives `ulimit -s unlimited`; the default
 # policy survives a 1 MiB stack) and showed why the lab handler printed nothing: pytest captures fd 2.  The report goes to a file now.
-#  B  destroy policy, lab build, SGA_DEBUG_SEGV=<file>: registers, code at rip, native frames, /proc/self/maps; SGA_CALL_LOG=<file>:
+#  B  destroy policy, lab build, SGA_DEBUG_SEGV=<file>: registers, native frames, /proc/self/maps; SGA_CALL_LOG=<file>:
 #     every C-ABI call of the process up to the crash (input of a Python-free replay)
 #  E  destroy policy with 4 hardware queues (the package's default is 2)
 #  F  destroy policy under MALLOC_CHECK_=3 HSA_ENABLE_INTERRUPT=0

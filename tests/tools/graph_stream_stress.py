@@ -1,8 +1,7 @@
 """Regression harness for "defect (a)" (DESIGN_EXPERIMENTS.md A.13), run as a SUBPROCESS by tests/test_gpu_graph_streams.py.
 
-The HIP runtime bundled with PyTorch-ROCm 2.10 (ROCm 7.0.2) overruns a graph's internal stream list inside hipGraphLaunch when ALL
-of the graph's internal streams share the LAUNCH stream's hardware queue; whether they do depends on which streams the process has
-created and destroyed before (a new stream takes the least-referenced hardware queue of its priority class).  This harness builds
+The HIP runtime bundled with PyTorch-ROCm 2.10 (ROCm 7.0.2) crashes in hipGraphLaunch on a normal-priority stream for some
+histories of streams that the process has created and destroyed before.  This harness builds
 such histories on purpose -- the pattern of scripts/r06/graph_stream_collision_repro.hip, which kills 7 of 64 masks with a
 normal-priority launch stream -- in a process that has PyTorch AND libsga_hip in it: for every mask, six normal-priority ballast
 streams are created and used, the masked ones destroyed, and a fresh handle runs 110 iterations (three fork-point candidates are
