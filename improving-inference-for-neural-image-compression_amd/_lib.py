@@ -18,7 +18,7 @@ LAB_LIB_PATH = os.path.join(_PKG_DIR, "libsga_hip_lab.so")
 PRODUCT_ENV_KNOBS = ("SGA_PRECISION", "SGA_NO_GRAPH", "SGA_NO_OVERLAP", "SGA_NO_SPLITK", "SGA_FORK_NAME", "SGA_FORK_VERBOSE",
                      "SGA_PROFILE_BY_LAYER", "SGA_X3_FORK", "SGA_X3_VARIANTS")
 
-SGA_ABI_VERSION = 6
+SGA_ABI_VERSION = 7
 
 STATUS = {
     0: "SGA_OK", -1: "SGA_ERR_BAD_ARG", -2: "SGA_ERR_BAD_SHAPE", -3: "SGA_ERR_UNSUPPORTED",
@@ -121,6 +121,34 @@ SYMBOLS["sga_ec_z_symbols_centred"] = (_I, [_P, _P, _I64, _I, _P, _P, _P, _P])
 SYMBOLS["sga_ec_encode"] = (_I, [_P, _P, _I64, _I, _P, _P, _P, _I, _P, _I, _P, _P])
 SYMBOLS["sga_ec_compact"] = (_I, [_P, _I, _P, _P, _I, _P, _P])
 SYMBOLS["sga_ec_decode"] = (_I, [_P, _P, _P, _I, _P, _I64, _I, _P, _P, _P, _I, _P, _P, _P])
+
+
+
+class SgaDropout(C.Structure):
+    _fields_ = [("p", _D), ("seed", C.c_uint64), ("offset", C.c_uint64), ("state", _P)]
+
+
+class SgaLinear(C.Structure):
+    _fields_ = [("rows", _I64), ("in_features", C.c_int32), ("out_features", C.c_int32), ("dtype", C.c_int32), ("act", C.c_int32),
+                ("x", _P), ("ld_x", _I64), ("w", _P), ("ld_w", _I64), ("bias", _P), ("residual", _P), ("ld_residual", _I64),
+                ("out", _P), ("ld_out", _I64), ("pre", _P), ("g_out", _P), ("ld_g_out", _I64),
+                ("g_x", _P), ("g_w", _P), ("g_bias", _P), ("dropout", SgaDropout)]
+
+
+class SgaLayerNorm(C.Structure):
+    _fields_ = [("rows", _I64), ("cols", C.c_int32), ("dtype", C.c_int32), ("param_dtype", C.c_int32), ("eps", _F),
+                ("x", _P), ("ld_x", _I64), ("w", _P), ("b", _P), ("y", _P), ("mean", _P), ("rstd", _P),
+                ("g_y", _P), ("ld_g_y", _I64), ("g_add", _P), ("ld_g_add", _I64), ("g_x", _P), ("g_w", _P), ("g_b", _P)]
+
+
+ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}      # sga_act
+SYMBOLS["sga_op_linear_workspace"] = (_I, [_P, _I, _P])
+SYMBOLS["sga_op_linear_fwd"] = (_I, [_P, _P, _I64, _P])
+SYMBOLS["sga_op_linear_bwd"] = (_I, [_P, _P, _I64, _P])
+SYMBOLS["sga_op_layer_norm_workspace"] = (_I, [_P, _I, _P])
+SYMBOLS["sga_op_layer_norm_fwd"] = (_I, [_P, _P])
+SYMBOLS["sga_op_layer_norm_bwd"] = (_I, [_P, _P, _I64, _P])
+SYMBOLS["sga_op_dropout"] = (_I, [_P, _I64, _P, _I64, _P, _I64, _I64, _I, _P, _P])
 
 _lib = None
 _lab = None

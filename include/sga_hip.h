@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define SGA_ABI_VERSION 6
+#define SGA_ABI_VERSION 7
 
 typedef enum sga_status {
   SGA_OK = 0,
@@ -331,6 +331,86 @@ int sga_ec_compact(const uint8_t* slots, int slot_cap, const uint32_t* block_byt
 int sga_ec_decode(const uint8_t* in, const uint64_t* block_off, const uint32_t* block_bytes, int nblocks,
                   const int32_t* tab, int64_t n, int block, const uint32_t* cdf, const int32_t* lens, const int32_t* offs,
                   int stride, int32_t* sym, int32_t* bad, void* stream);
+
+/* ---- token blocks: operators over the rows of a matrix [rows, features] -----------------------------------------------
+ * What a transform or an entropy model built from token blocks over the latent grid needs next to the convolutions above:
+ * the matrix product with a fused epilogue, layer norm and counter-based dropout, each with its backward pass.  They follow
+ * the sga_ec_* convention: no handle, plain DEVICE pointers, the caller's stream (of the current device), asynchronous, no
+ * allocation, no state kept between calls -- a workspace, where one is asked for, belongs to the call until the stream has
+ * passed it; calls that may run at the same time (two streams, two captured graphs) take one each.  Every sum, statistic and
+ * activation is computed in float32 and rounded once to `dtype` on store.  A row starts every `ld` ELEMENTS (rows of a wider
+ * buffer; 0 repeats one row, inputs only), its elements are adjacent; no alignment beyond the element's own is required.
+ * rows = 0 is a call without output (weight gradients: zeros).  Outputs must not overlap inputs, except where said. */
+typedef enum sga_dtype { SGA_DTYPE_F32 = 0, SGA_DTYPE_BF16 = 1, SGA_DTYPE_F16 = 2 } sga_dtype;
+typedef enum sga_act {
+  SGA_ACT_NONE = 0,
+  SGA_ACT_RELU = 1,
+  SGA_ACT_GELU = 2,       /* z Phi(z), Phi the normal distribution function           */
+  SGA_ACT_GELU_TANH = 3,  /* z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2           */
+  SGA_ACT_SILU = 4        /* z / (1 + exp(-z))                                         */
+} sga_act;
+
+/* Dropout D_p: element i = row * features + column is kept and scaled by 1 / (1 - p), or 0 (also where it is inf / NaN).  It is
+ * kept if word i % 4 of Philox4x32-10 with counter (i/4 low, i/4 high, offset low, offset high) and key (seed low, seed high)
+ * is >= round(p * 2^32).  The mask is a function of (seed, offset, i): it is never stored, the backward pass draws it
+ * again.  `state` (optional, DEVICE, 8-byte aligned): {seed, offset} read when the kernel runs, in place of the members -- a
+ * captured graph takes new numbers at every replay that way.  p = 0: no dropout, p = 1: nothing is kept. */
+typedef struct sga_dropout {
+  double p;
+  uint64_t seed, offset;
+  const uint64_t* state;
+} sga_dropout;
+
+/* out = residual + D_p(act(z)),  z = x w^T + bias:  x [rows, in_features], w [out_features, in_features], bias [out_features] or
+ * NULL, residual [rows, out_features] or NULL; pre (optional, forward: written; backward: read unless act is NONE) receives
+ * z [rows, out_features], contiguous.  Backward: dz = D_p(g_out) act'(pre) (of act = RELU: 0 at 0), rounded to `dtype` as the
+ * operand of g_x [rows, in_features] = dz w and g_w [out_features, in_features] = dz^T x; g_bias [out_features] = sum of dz over
+ * rows.  g_x, g_w, g_bias are contiguous, any of them NULL = not wanted; the gradient of `residual` is g_out itself.
+ * residual may be out itself (same ld).  Limits: in_features, out_features <= 2^20, rows < 2^31. */
+typedef struct sga_linear {
+  int64_t rows;
+  int32_t in_features, out_features, dtype, act;
+  const void* x;        int64_t ld_x;
+  const void* w;        int64_t ld_w;
+  const void* bias;
+  const void* residual; int64_t ld_residual;
+  void* out;            int64_t ld_out;
+  void* pre;
+  const void* g_out;    int64_t ld_g_out;
+  void* g_x; void* g_w; void* g_bias;
+  sga_dropout dropout;
+} sga_linear;
+/* bytes of DEVICE workspace (256-byte aligned) that the call with exactly these members needs; may be 0 */
+int sga_op_linear_workspace(const sga_linear* a, int backward, int64_t* bytes);
+int sga_op_linear_fwd(const sga_linear* a, void* workspace, int64_t workspace_bytes, void* stream);
+int sga_op_linear_bwd(const sga_linear* a, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* y = (x - mean) rstd w + b per row of x [rows, cols], rstd = 1 / sqrt(var + eps), var the mean of (x - mean)^2 (two passes over
+ * the row on chip); w, b [cols] of type param_dtype (dtype or F32), NULL = 1 and 0.  mean, rstd [rows] float32: written by the
+ * forward pass (NULL = not wanted), read by the backward pass:  g = g_y w, h = (x - mean) rstd,
+ * g_x = g_add + rstd (g - mean(g) - h mean(g h)), g_w = sum of g_y h, g_b = sum of g_y over rows.  g_add [rows, cols]
+ * (optional): the gradient that reaches x past the norm.  y, g_x, g_w, g_b contiguous, any of g_x, g_w, g_b NULL = not
+ * wanted.  Limits: cols <= 2^20, rows < 2^31. */
+typedef struct sga_layer_norm {
+  int64_t rows;
+  int32_t cols, dtype, param_dtype;
+  float eps;
+  const void* x;     int64_t ld_x;
+  const void* w; const void* b;
+  void* y;
+  float* mean; float* rstd;
+  const void* g_y;   int64_t ld_g_y;
+  const void* g_add; int64_t ld_g_add;
+  void* g_x; void* g_w; void* g_b;
+} sga_layer_norm;
+int sga_op_layer_norm_workspace(const sga_layer_norm* a, int backward, int64_t* bytes);
+int sga_op_layer_norm_fwd(const sga_layer_norm* a, void* stream);
+int sga_op_layer_norm_bwd(const sga_layer_norm* a, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* y = residual + D_p(x) over [rows, cols] (residual NULL = 0; y contiguous; y may be x or residual if that is contiguous too).
+ * Its backward pass is the same call on the gradient, without residual. */
+int sga_op_dropout(const void* x, int64_t ld_x, const void* residual, int64_t ld_residual, void* y, int64_t rows, int64_t cols,
+                   int dtype, const sga_dropout* dropout, void* stream);
 
 /* ---- measurement: per-kernel hipEvent timing of the convolution launches -------------------
  * Between sga_profile_begin and sga_profile_end every MFMA convolution launch issued through

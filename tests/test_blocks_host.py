@@ -1,0 +1,149 @@
+"""CPU tests of the token-block operators' argument checks (sga_amd.blocks and the C entry points): a call that cannot be carried
+out is refused before anything is launched."""
+import ctypes as C
+
+import pytest
+import torch
+
+import sga_amd  # noqa: F401
+from sga_amd import _lib, blocks
+
+P = 1 << 20      # an address that no check reads
+
+
+def linear(**kw):
+    a = _lib.SgaLinear(rows=4, in_features=8, out_features=16, dtype=1, act=0, x=P, ld_x=8, w=P, ld_w=8, out=P, ld_out=16, ld_residual=16,
+                       g_out=P, ld_g_out=16, g_x=P, g_w=P, g_bias=P)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+BAD, UNSUPPORTED = -1, -3
+
+
+@pytest.mark.parametrize("change,status", [
+    ({"rows": -1}, BAD), ({"in_features": 0}, BAD), ({"out_features": 0}, BAD), ({"dtype": 3}, BAD), ({"dtype": -1}, BAD), ({"act": 5}, BAD),
+    ({"ld_x": 7}, BAD), ({"ld_x": -8}, BAD), ({"ld_w": 4}, BAD), ({"x": P + 1}, BAD), ({"w": P + 1}, BAD),
+    ({"in_features": (1 << 20) + 1, "ld_x": 1 << 21, "ld_w": 1 << 21}, UNSUPPORTED), ({"rows": 1 << 31}, UNSUPPORTED),
+    ({"dropout": _lib.SgaDropout(-0.1, 0, 0, None)}, BAD), ({"dropout": _lib.SgaDropout(1.1, 0, 0, None)}, BAD),
+    ({"dropout": _lib.SgaDropout(float("nan"), 0, 0, None)}, BAD), ({"dropout": _lib.SgaDropout(0.5, 0, 0, P + 4)}, BAD)])
+def test_linear_refuses(change, status):
+    lib = _lib.load_library()
+    n = C.c_int64(0)
+    for backward in (0, 1):
+        assert lib.sga_op_linear_workspace(C.byref(linear(**change)), backward, C.byref(n)) == status
+    assert lib.sga_op_linear_fwd(C.byref(linear(**change)), None, 0, None) == status
+    assert lib.sga_op_linear_bwd(C.byref(linear(**change)), None, 0, None) == status
+
+
+@pytest.mark.parametrize("change", [{"x": None}, {"w": None}, {"out": None}, {"ld_out": 15}, {"ld_out": 0}, {"residual": P, "ld_residual": 3},
+                                    {"bias": P + 1}, {"residual": P + 1}, {"out": P + 1}])
+def test_linear_forward_refuses(change):
+    assert _lib.load_library().sga_op_linear_fwd(C.byref(linear(**change)), None, 0, None) == BAD
+
+
+@pytest.mark.parametrize("change", [{"g_out": None}, {"act": 2}, {"x": None}, {"w": None}, {"ld_g_out": 15}, {"g_x": P + 1}, {"g_bias": P + 1}])
+def test_linear_backward_refuses(change):
+    assert _lib.load_library().sga_op_linear_bwd(C.byref(linear(**change)), P, 1 << 30, None) == BAD
+
+
+def test_linear_refuses_null_and_small_workspaces():
+    lib = _lib.load_library()
+    n = C.c_int64(0)
+    assert lib.sga_op_linear_workspace(None, 0, C.byref(n)) == BAD
+    assert lib.sga_op_linear_workspace(C.byref(linear()), 0, None) == BAD
+    assert lib.sga_op_linear_fwd(None, None, 0, None) == BAD
+    a = linear(act=2, pre=P)
+    assert lib.sga_op_linear_workspace(C.byref(a), 1, C.byref(n)) == 0 and n.value > 0
+    assert lib.sga_op_linear_bwd(C.byref(a), P, n.value - 1, None) == BAD
+    assert lib.sga_op_linear_bwd(C.byref(a), None, n.value, None) == BAD
+    assert lib.sga_op_linear_bwd(C.byref(a), P + 8, n.value, None) == BAD
+
+
+def norm(**kw):
+    a = _lib.SgaLayerNorm(rows=4, cols=8, dtype=1, param_dtype=0, eps=1e-5, x=P, ld_x=8, y=P, mean=P, rstd=P, g_y=P, ld_g_y=8, g_x=P, g_w=P, g_b=P)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("change,status", [
+    ({"rows": -1}, BAD), ({"cols": 0}, BAD), ({"dtype": 3}, BAD), ({"param_dtype": 2}, BAD), ({"ld_x": 7}, BAD), ({"x": P + 1}, BAD), ({"w": P + 2}, BAD),
+    ({"x": None}, BAD), ({"mean": P + 2}, BAD), ({"cols": (1 << 20) + 1, "ld_x": 1 << 21}, UNSUPPORTED), ({"rows": 1 << 31}, UNSUPPORTED)])
+def test_layer_norm_refuses(change, status):
+    lib = _lib.load_library()
+    n = C.c_int64(0)
+    for backward in (0, 1):
+        assert lib.sga_op_layer_norm_workspace(C.byref(norm(**change)), backward, C.byref(n)) == status
+    assert lib.sga_op_layer_norm_fwd(C.byref(norm(**change)), None) == status
+    assert lib.sga_op_layer_norm_bwd(C.byref(norm(**change)), P, 1 << 30, None) == status
+
+
+def test_layer_norm_refuses_by_direction():
+    lib = _lib.load_library()
+    n = C.c_int64(0)
+    for change in ({"eps": -1.0}, {"eps": float("nan")}, {"y": None}, {"y": P + 1}):
+        assert lib.sga_op_layer_norm_fwd(C.byref(norm(**change)), None) == BAD
+    for change in ({"g_y": None}, {"mean": None}, {"rstd": None}, {"ld_g_y": 3}, {"g_add": P, "ld_g_add": 3}, {"g_x": P + 1}, {"g_w": P + 2}):
+        assert lib.sga_op_layer_norm_bwd(C.byref(norm(**change)), P, 1 << 30, None) == BAD
+    assert lib.sga_op_layer_norm_workspace(C.byref(norm()), 1, C.byref(n)) == 0 and n.value > 0
+    assert lib.sga_op_layer_norm_bwd(C.byref(norm()), P, n.value - 1, None) == BAD
+    assert lib.sga_op_layer_norm_bwd(C.byref(norm()), None, 0, None) == BAD
+
+
+def test_dropout_refuses():
+    lib = _lib.load_library()
+
+    def call(x=P, ld_x=8, res=None, ld_res=8, y=P, rows=4, cols=8, dtype=1, p=0.5, state=None, drop=True):
+        d = _lib.SgaDropout(p, 1, 0, state)
+        return lib.sga_op_dropout(x, ld_x, res, ld_res, y, rows, cols, dtype, C.byref(d) if drop else None, None)
+
+    for kw in ({"x": None}, {"y": None}, {"ld_x": 7}, {"res": P, "ld_res": 7}, {"rows": -1}, {"cols": 0}, {"dtype": 3}, {"p": -1.0}, {"p": 2.0},
+               {"state": P + 1}, {"drop": False}, {"x": P + 1}, {"y": P + 1}, {"res": P + 1}):
+        assert call(**kw) == BAD, kw
+    assert call(rows=1 << 31) == UNSUPPORTED
+    assert call(x=None, y=None, rows=0) == 0
+
+
+def test_python_refuses_before_it_asks_for_a_gpu():
+    x, w = torch.ones(4, 8), torch.ones(16, 8)
+    with pytest.raises(ValueError, match="on the GPU"):
+        blocks.linear(x, w)
+    with pytest.raises(TypeError):
+        blocks.linear(x.double(), w)
+    with pytest.raises(TypeError):
+        blocks.linear([1.0], w)
+    with pytest.raises(ValueError, match="adjacent"):
+        blocks.layer_norm(torch.ones(8, 4).t())
+    with pytest.raises(ValueError, match="common stride"):
+        blocks.layer_norm(torch.ones(4, 6, 8)[:, ::2][:3, :2])
+    with pytest.raises(ValueError, match="overlap"):
+        blocks.layer_norm(torch.ones(100).as_strided((4, 8), (3, 1)))
+    with pytest.raises(ValueError, match="at least one feature"):
+        blocks.layer_norm(torch.ones(4, 0))
+    with pytest.raises(ValueError, match="at least one feature"):
+        blocks.dropout(torch.tensor(1.0), 0.5, 1)
+    with pytest.raises(ValueError, match="act"):
+        blocks._act("tanh")
+    for bad in ((-0.5, 1, 0), (1.5, 1, 0), (float("nan"), 1, 0), (0.5, 1), (0.5, torch.zeros(2))):
+        with pytest.raises(ValueError):
+            blocks._drop(bad, torch.device("cpu"))
+    d = blocks._drop((0.5, -1, 1 << 65), torch.device("cpu"))
+    assert d.seed == (1 << 64) - 1 and d.offset == 0
+
+
+def test_row_layouts():
+    """Rows of wider buffers, repeated rows and batches collapse to (rows, features, row stride); checked up to the device."""
+    def layout(t):
+        try:
+            blocks._rows(t, "t")
+        except ValueError as e:
+            return "GPU" in str(e)      # everything but the device is in order
+        raise AssertionError
+    base = torch.ones(6, 40)
+    for t in (base, base[:, 3:20], base[::2], base[:1].expand(5, 40), base.view(2, 3, 40), base.view(2, 3, 40)[:, :, :8], torch.ones(8), base[:, :1],
+              torch.ones(0, 8), base[2:3, 1:9], base.view(2, 3, 40)[:1, ::2]):
+        assert layout(t), t.shape
+    for t in (base.t(), base.view(2, 3, 40)[:, :2], base.expand(3, 6, 40)):
+        assert not layout(t), t.shape
