@@ -17,32 +17,73 @@ __device__ __forceinline__ float to_f32(f16 v) { return (float)v; }
 // the one rounding of a result: to nearest, ties to even
 template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }
 
-__device__ __forceinline__ float act_value(float z, int act) {
-  switch (act) {
-    case SGA_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
-    case SGA_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case SGA_ACT_GELU_TANH: return 0.5f * z * (1.f + tanhf(0.79788456080286536f * fmaf(0.044715f * z * z, z, z)));
-    case SGA_ACT_SILU: return z / (1.f + expf(-z));
-    default: return z;
-  }
+// e^x to 2 units in the last place: 2^(x log2 e) by the hardware's exp2, and the part of x log2 e that float32 cannot hold as a
+// factor.  The clamp keeps infinities out of that part; a NaN becomes some number, every use multiplies by x again.
+__device__ __forceinline__ float exp_f(float x) {
+  x = fminf(fmaxf(x, -1000.f), 1000.f);
+  const float t = x * 1.44269504f;
+  const float e = fmaf(x, 1.925963033e-8f, fmaf(x, 1.44269504f, -t));
+  return __builtin_amdgcn_exp2f(t) * fmaf(e, 0.69314718f, 1.f);
+}
+// 1 / (1 + e^-x)
+__device__ __forceinline__ float sigmoid_f(float x) { return __builtin_amdgcn_rcpf(1.f + exp_f(-x)); }
+
+// Phi(-|z|) = erfc(|z| / sqrt 2) / 2 = g(|z|) e^(-z^2 / 2) with g smooth and slowly varying: g as a polynomial of degree 8 in
+// t = 1 / (1 + 0.3 |z|), fitted on 0 <= |z| <= 14 for the least maximum of the relative error (5.8e-8 in exact arithmetic, 5e-7 with
+// float32 steps; beyond 14 the exponential is 0).  Relative accuracy in the tail is what 1 + erf(z) cannot give, and the
+// backward pass shares the exponential: 8 + 10 instructions where the library's erf and exp take about 60.
+__device__ __forceinline__ float normal_tail(float z, float gauss) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.3f, 1.f));
+  float p = 0.038378264755010605f;
+  p = fmaf(p, t, -0.16916599869728088f);
+  p = fmaf(p, t, 0.22865986824035645f);
+  p = fmaf(p, t, -0.07650627195835114f);
+  p = fmaf(p, t, 0.14253540337085724f);
+  p = fmaf(p, t, 0.09468357264995575f);
+  p = fmaf(p, t, 0.12192033231258392f);
+  p = fmaf(p, t, 0.1194876879453659f);
+  p = fmaf(p, t, 7.168815500335768e-06f);
+  return p * gauss;
 }
 
-__device__ __forceinline__ float act_slope(float z, int act) {
-  switch (act) {
-    case SGA_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-    case SGA_ACT_GELU:
-      return fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678118654752f)));
-    case SGA_ACT_GELU_TANH: {
-      const float t = tanhf(0.79788456080286536f * fmaf(0.044715f * z * z, z, z));
-      const float c = fminf(fmaxf(z, -16.f), 16.f);      // beyond, 1 - t^2 is 0 and the polynomial must not be inf
-      return 0.5f * (1.f + t) + 0.5f * c * (1.f - t * t) * 0.79788456080286536f * fmaf(0.134145f * c, c, 1.f);
-    }
-    case SGA_ACT_SILU: {
-      const float s = 1.f / (1.f + expf(-z));
-      return s * fmaf(z, 1.f - s, 1.f);
-    }
-    default: return 1.f;
+template <int ACT> __device__ __forceinline__ float act_value_of(float z) {
+  if constexpr (ACT == SGA_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
+  if constexpr (ACT == SGA_ACT_GELU) {
+    const float q = normal_tail(z, exp_f(-0.5f * z * z));
+    return z * (z > 0.f ? 1.f - q : q);
   }
+  if constexpr (ACT == SGA_ACT_GELU_TANH) return z * sigmoid_f(1.59576912160573072f * fmaf(0.044715f * z * z, z, z));
+  if constexpr (ACT == SGA_ACT_SILU) return z * sigmoid_f(z);
+  return z;
+}
+template <int ACT> __device__ __forceinline__ float act_slope_of(float z) {
+  if constexpr (ACT == SGA_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  if constexpr (ACT == SGA_ACT_GELU) {
+    const float gauss = exp_f(-0.5f * z * z), q = normal_tail(z, gauss);
+    return fmaf(z * 0.39894228040143268f, gauss, z > 0.f ? 1.f - q : q);
+  }
+  if constexpr (ACT == SGA_ACT_GELU_TANH) {
+    const float e = exp_f(-1.59576912160573072f * fmaf(0.044715f * z * z, z, z)), s = __builtin_amdgcn_rcpf(1.f + e);
+    const float c = fminf(fmaxf(z, -16.f), 16.f);      // s (1 - s) is 0 beyond, and the polynomial must not be inf
+    const float d = s * (s > 0.f ? e * s : 0.f);       // s (1 - s) without the difference
+    return fmaf(c * d, 1.59576912160573072f * fmaf(0.134145f * c, c, 1.f), s) + (z - z);
+  }
+  if constexpr (ACT == SGA_ACT_SILU) {
+    const float e = exp_f(-z), s = __builtin_amdgcn_rcpf(1.f + e);
+    return s > 0.f ? s * fmaf(z, e * s, 1.f) : (z - z);
+  }
+  return 1.f;
+}
+// v[j] = act(v[j]); g[j] *= act'(v[j])
+template <int N> __device__ __forceinline__ void act_values(float v[N], int act) {
+#define EACH(A) case A: _Pragma("unroll") for (int j = 0; j < N; ++j) v[j] = act_value_of<A>(v[j]); break
+  switch (act) { EACH(SGA_ACT_RELU); EACH(SGA_ACT_GELU); EACH(SGA_ACT_GELU_TANH); EACH(SGA_ACT_SILU); default: break; }
+#undef EACH
+}
+template <int N> __device__ __forceinline__ void act_slopes(float g[N], const float v[N], int act) {
+#define EACH(A) case A: _Pragma("unroll") for (int j = 0; j < N; ++j) g[j] *= act_slope_of<A>(v[j]); break
+  switch (act) { EACH(SGA_ACT_RELU); EACH(SGA_ACT_GELU); EACH(SGA_ACT_GELU_TANH); EACH(SGA_ACT_SILU); default: break; }
+#undef EACH
 }
 
 // Dropout as the kernels take it.  keep: word >= thr (thr = round(p 2^32), up to 2^32: nothing is kept); on = 0: no dropout.
@@ -95,5 +136,114 @@ inline bool dtype_ok(int t) { return t == SGA_DTYPE_F32 || t == SGA_DTYPE_BF16 |
 inline bool at_ok(const void* p, int dtype) { return ((uintptr_t)p & (dtype_bytes(dtype) - 1)) == 0; }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+
+// ---- epilogue of a product: 8 adjacent columns of one row ----------------------------------------------------------------
+struct Epilogue {
+  const void* bias; const void* residual; int64_t ld_residual; void* out; int64_t ld_out; void* pre; int64_t cols; int act;
+  int vec;       // every row piece of 8 columns is whole and 16-byte aligned in every tensor
+  Drop drop;
+};
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// 8 adjacent elements, 16-byte aligned
+__device__ __forceinline__ void load8(const float* p, float v[8]) {
+  const f32x4 a = ((const f32x4*)p)[0], b = ((const f32x4*)p)[1];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+}
+template <typename T> __device__ __forceinline__ void load8(const T* p, float v[8]) {
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  const t8 a = *(const t8*)p;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = (float)a[j];
+}
+__device__ __forceinline__ void store8(float* p, const float v[8]) {
+  ((f32x4*)p)[0] = f32x4{v[0], v[1], v[2], v[3]};
+  ((f32x4*)p)[1] = f32x4{v[4], v[5], v[6], v[7]};
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const float v[8]) {
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  t8 a;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a[j] = from_f32<T>(v[j]);
+  *(t8*)p = a;
+}
+
+// columns n .. n + 7 of row m (those below e.cols); seed / offset: drop_key's
+template <typename T>
+__device__ __forceinline__ void epilogue8(const Epilogue& e, uint64_t seed, uint64_t offset, int64_t m, int64_t n, float v[8]) {
+  T* out = (T*)e.out + m * e.ld_out + n;
+  const T* res = e.residual ? (const T*)e.residual + m * e.ld_residual + n : nullptr;
+  T* pre = e.pre ? (T*)e.pre + m * e.cols + n : nullptr;
+  const T* bias = e.bias ? (const T*)e.bias + n : nullptr;
+  if (e.vec) {
+    if (n >= e.cols) return;
+    if (bias) {
+      float b[8];
+      load8(bias, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += b[j];
+    }
+    if (pre) store8(pre, v);
+    act_values<8>(v, e.act);
+    if (e.drop.on) {
+      const uint64_t g = (uint64_t)(m * e.cols + n) >> 2;      // cols and n are multiples of 8 here
+      uint32_t w[8];
+      drop_words(seed, offset, g, w);
+      drop_words(seed, offset, g + 1, w + 4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = drop_apply(e.drop, w[j], v[j]);
+    }
+    if (res) {
+      float r[8];
+      load8(res, r);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += r[j];
+    }
+    store8(out, v);
+    return;
+  }
+  // pieces of any length and alignment, element by element; the 8 elements' words lie in three groups of four at most
+  const int live = e.cols - n < 8 ? (int)(e.cols - n) : 8;
+  uint32_t w[12];
+  const uint64_t i0 = (uint64_t)(m * e.cols + n);
+  const int shift = (int)(i0 & 3);
+  if (e.drop.on) {
+#pragma unroll
+    for (int g = 0; g < 3; ++g) drop_words(seed, offset, (i0 >> 2) + g, w + 4 * g);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < live) {
+      if (bias) v[j] += to_f32(bias[j]);
+      if (pre) pre[j] = from_f32<T>(v[j]);
+    }
+  act_values<8>(v, e.act);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < live) {
+      float u = v[j];
+      if (e.drop.on) u = drop_apply(e.drop, shift == 0 ? w[j] : shift == 1 ? w[j + 1] : shift == 2 ? w[j + 2] : w[j + 3], u);
+      if (res) u += to_f32(res[j]);
+      out[j] = from_f32<T>(u);
+    }
+}
+
+// ---- C[m, n] = epilogue(sum_k X(m, k) W(n, k)) (token_product.hip) -------------------------------------------------------
+// strided = 0: operand(r, k) = p[r ld + k]; strided = 1: operand(r, k) = p[k ld + r]
+// padded: rows (as they lie) are followed by zeros up to the next 16 bytes
+struct Operand { const void* p; int64_t ld; int strided; int padded; };
+struct Product {
+  Operand x, w;
+  int64_t M, N, K;
+  int dtype;
+  Epilogue e;
+};
+// device workspace (bytes) of launch_product with these members, and the launch itself: 0 or an sga_status
+int64_t product_workspace(const Product& p);
+int launch_product(const Product& p, char* ws, hipStream_t st);
 
 }  // namespace token

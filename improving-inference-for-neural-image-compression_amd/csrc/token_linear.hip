@@ -7,78 +7,64 @@ using namespace token;
 
 namespace {
 
-struct Epilogue {
-  const void* bias; const void* residual; int64_t ld_residual; void* out; int64_t ld_out; void* pre; int64_t cols; int act; Drop drop;
-};
-
-template <typename T>
-__device__ __forceinline__ void epilogue_one(const Epilogue& e, uint64_t seed, uint64_t offset, int64_t m, int64_t n, float v) {
-  if (e.bias) v += to_f32(((const T*)e.bias)[n]);
-  if (e.pre) ((T*)e.pre)[m * e.cols + n] = from_f32<T>(v);
-  v = act_value(v, e.act);
-  if (e.drop.on) v = drop_one(e.drop, seed, offset, (uint64_t)(m * e.cols + n), v);
-  if (e.residual) v += to_f32(((const T*)e.residual)[m * e.ld_residual + n]);
-  ((T*)e.out)[m * e.ld_out + n] = from_f32<T>(v);
-}
-
-// C[m, n] = epi(sum_k A(m, k) B(n, k)), A(m, k) = A[m sam + k sak]: one 64 x 64 tile per workgroup, 4 x 4 results per lane
-template <typename T>
-__global__ __launch_bounds__(256) void token_product_kernel(const T* __restrict__ A, int64_t sam, int64_t sak, const T* __restrict__ B,
-                                                            int64_t sbn, int64_t sbk, int64_t M, int64_t N, int64_t K, const Epilogue e) {
-  __shared__ float As[16][65], Bs[16][65];
-  const int64_t m0 = (int64_t)blockIdx.x * 64, n0 = (int64_t)blockIdx.y * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < K; k0 += 16) {
-    for (int i = threadIdx.x; i < 1024; i += 256) {
-      const int k = i & 15, r = i >> 4;
-      const bool ink = k0 + k < K;
-      As[k][r] = ink && m0 + r < M ? to_f32(A[(m0 + r) * sam + (k0 + k) * sak]) : 0.f;
-      Bs[k][r] = ink && n0 + r < N ? to_f32(B[(n0 + r) * sbn + (k0 + k) * sbk]) : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      float a[4], b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { a[i] = As[k][ty * 4 + i]; b[i] = Bs[k][tx * 4 + i]; }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
-    }
-    __syncthreads();
-  }
-  uint64_t seed = 0, offset = 0;
-  if (e.drop.on) drop_key(e.drop, seed, offset);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-      if (m < M && n < N) epilogue_one<T>(e, seed, offset, m, n, acc[i][j]);
-    }
-}
-
-
-// dz = D_p(g) act'(pre) (dz null: not wanted), part[chunk][n] = sum of the chunk's dz (part null: not wanted)
+// dz = D_p(g) act'(pre) (dz null: not wanted; its rows end in zeros up to ld_dz), part[chunk][n] = sum of the chunk's dz before the
+// rounding (part null: not wanted).  32 pieces of 8 columns x 8 rows per workgroup; `vec`: all pieces whole and 16-byte aligned.
 template <typename T>
 __global__ __launch_bounds__(256) void token_dz_kernel(const T* __restrict__ g, int64_t ld_g, const T* __restrict__ pre, int act, const Drop d,
-                                                       T* __restrict__ dz, float* __restrict__ part, int64_t rows, int64_t cols, int64_t per) {
-  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (n >= cols) return;
+                                                       T* __restrict__ dz, int64_t ld_dz, float* __restrict__ part, int64_t rows, int64_t cols,
+                                                       int64_t per, int vec) {
+  __shared__ float sh[8][264];
+  const int px = threadIdx.x & 31, py = threadIdx.x >> 5;
+  const int64_t n = (int64_t)blockIdx.x * 256 + px * 8;
   const int64_t m0 = (int64_t)blockIdx.y * per, m1 = m0 + per < rows ? m0 + per : rows;
+  const int live = cols - n >= 8 ? 8 : cols > n ? (int)(cols - n) : 0;
   uint64_t seed = 0, offset = 0;
   if (d.on) drop_key(d, seed, offset);
-  float sum = 0.f;
-  for (int64_t m = m0; m < m1; ++m) {
-    float v = to_f32(g[m * ld_g + n]);
-    if (d.on) v = drop_one(d, seed, offset, (uint64_t)(m * cols + n), v);
-    if (act != SGA_ACT_NONE) v *= act_slope(to_f32(pre[m * cols + n]), act);
-    sum += v;
-    if (dz) dz[m * cols + n] = from_f32<T>(v);
+  float sum[8] = {};
+  for (int64_t m = m0 + py; m < m1 && live > 0; m += 8) {
+    float v[8], z[8];
+    if (vec) {
+      load8(g + m * ld_g + n, v);
+      if (act != SGA_ACT_NONE) load8(pre + m * cols + n, z);
+      if (d.on) {
+        uint32_t w[8];
+        const uint64_t q = (uint64_t)(m * cols + n) >> 2;
+        drop_words(seed, offset, q, w);
+        drop_words(seed, offset, q + 1, w + 4);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = drop_apply(d, w[j], v[j]);
+      }
+    } else {
+      uint32_t w[12];
+      const uint64_t i0 = (uint64_t)(m * cols + n);
+      const int shift = (int)(i0 & 3);
+      if (d.on) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) drop_words(seed, offset, (i0 >> 2) + k, w + 4 * k);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = j < live ? to_f32(g[m * ld_g + n + j]) : 0.f;
+        z[j] = j < live && act != SGA_ACT_NONE ? to_f32(pre[m * cols + n + j]) : 0.f;
+        if (d.on) v[j] = j < live ? drop_apply(d, shift == 0 ? w[j] : shift == 1 ? w[j + 1] : shift == 2 ? w[j + 2] : w[j + 3], v[j]) : 0.f;
+      }
+    }
+    act_slopes<8>(v, z, act);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[j] += v[j];
+    if (dz) store8(dz + m * ld_dz + n, v);      // ld_dz is a multiple of 8: a ragged last piece ends in zeros
   }
-  if (part) part[(int64_t)blockIdx.y * cols + n] = sum;
+  if (!part) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sh[py][px * 8 + j] = sum[j];
+  __syncthreads();
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c < cols) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += sh[k][threadIdx.x];
+    part[(int64_t)blockIdx.y * cols + c] = s;
+  }
 }
 
 template <typename T>
@@ -93,19 +79,58 @@ __global__ __launch_bounds__(256) void token_sum_parts_kernel(const float* __res
 constexpr int kMaxFeatures = 1 << 20;
 constexpr int64_t kMaxRows = 0x7fffffff;
 
-// what the backward pass lays out in its workspace
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+Product forward_product(const sga_linear& a) {
+  const int64_t E = (int64_t)dtype_bytes(a.dtype);
+  Product p = {};
+  p.x = {a.x, a.ld_x, 0, 0};
+  p.w = {a.w, a.ld_w, 0, 0};
+  p.M = a.rows; p.N = a.out_features; p.K = a.in_features;
+  p.dtype = a.dtype;
+  p.e = {a.bias, a.residual, a.ld_residual, a.out, a.ld_out, a.pre, a.out_features, a.act, 0, make_drop(a.dropout)};
+  p.e.vec = a.out_features % 8 == 0 && aligned16(a.out) && a.ld_out * E % 16 == 0 && aligned16(a.bias) && aligned16(a.pre) &&
+            (!a.residual || (aligned16(a.residual) && a.ld_residual * E % 16 == 0));
+  return p;
+}
+
+// what the backward pass lays out in its workspace: [dz][parts of g_bias][the products' own], the two products one after the other
 struct BwdPlan {
   bool dz, part;             // dz differs from g_out; g_bias is wanted
-  int64_t per, chunks, dz_off, part_off, bytes;
+  int64_t ld_dz, per, chunks, dz_off, part_off, prod_off, bytes;
+  Product gx, gw;
 };
-BwdPlan bwd_plan(const sga_linear& a) {
+BwdPlan bwd_plan(const sga_linear& a, char* ws) {
+  const int64_t E = (int64_t)dtype_bytes(a.dtype);
   BwdPlan p = {};
   p.dz = (a.act != SGA_ACT_NONE || a.dropout.p > 0.0) && (a.g_x || a.g_w);
   p.part = a.g_bias != nullptr;
+  p.ld_dz = round_up(a.out_features, 8);
   p.per = ceil_div(a.rows, 1024) > 64 ? ceil_div(a.rows, 1024) : 64;      // rows per partial sum of g_bias: at most 1024 of them
   p.chunks = ceil_div(a.rows, p.per);
-  if (p.dz) { p.dz_off = p.bytes; p.bytes += round_up(a.rows * a.out_features * (int64_t)dtype_bytes(a.dtype), 256); }
+  if (p.dz) { p.dz_off = p.bytes; p.bytes += round_up(a.rows * p.ld_dz * E, 256); }
   if (p.part) { p.part_off = p.bytes; p.bytes += round_up(p.chunks * a.out_features * 4, 256); }
+  p.prod_off = p.bytes;
+  Operand dz = {a.g_out, a.ld_g_out, 0, 0};
+  if (p.dz) dz = {ws + p.dz_off, p.ld_dz, 0, 1};
+  Epilogue e = {};
+  e.cols = e.ld_out = a.in_features;
+  int64_t most = 0;
+  if (a.g_x && a.rows > 0) {
+    e.out = a.g_x;
+    e.vec = a.in_features % 8 == 0 && aligned16(a.g_x);
+    p.gx = {dz, {a.w, a.ld_w, 1, 0}, a.rows, a.in_features, a.out_features, a.dtype, e};
+    most = product_workspace(p.gx);
+  }
+  if (a.g_w) {
+    e.out = a.g_w;
+    e.vec = a.in_features % 8 == 0 && aligned16(a.g_w);
+    dz.strided = 1;
+    p.gw = {dz, {a.x, a.ld_x, 1, 0}, a.out_features, a.in_features, a.rows, a.dtype, e};
+    const int64_t b = product_workspace(p.gw);
+    most = most > b ? most : b;
+  }
+  p.bytes += most;
   return p;
 }
 
@@ -138,50 +163,27 @@ int bwd_check(const sga_linear* a) {
 #define LAUNCHED() do { if (hipGetLastError() != hipSuccess) return SGA_ERR_HIP; } while (0)
 
 template <typename T>
-int product(const void* A, int64_t sam, int64_t sak, const void* B, int64_t sbn, int64_t sbk, int64_t M, int64_t N, int64_t K, const Epilogue& e,
-            hipStream_t st) {
-  hipLaunchKernelGGL((token_product_kernel<T>), dim3((unsigned)ceil_div(M, 64), (unsigned)ceil_div(N, 64)), dim3(256), 0, st, (const T*)A, sam, sak,
-                     (const T*)B, sbn, sbk, M, N, K, e);
-  LAUNCHED();
-  return SGA_OK;
-}
-
-template <typename T>
-int linear_fwd(const sga_linear& a, hipStream_t st) {
-  Epilogue e = {a.bias, a.residual, a.ld_residual, a.out, a.ld_out, a.pre, a.out_features, a.act, make_drop(a.dropout)};
-  return product<T>(a.x, a.ld_x, 1, a.w, a.ld_w, 1, a.rows, a.out_features, a.in_features, e, st);
-}
-
-template <typename T>
 int linear_bwd(const sga_linear& a, char* ws, hipStream_t st) {
-  const BwdPlan p = bwd_plan(a);
-  const T* dz = (const T*)a.g_out;
-  int64_t ld_dz = a.ld_g_out;
+  const BwdPlan p = bwd_plan(a, ws);
+  const int64_t E = sizeof(T);
   float* part = p.part ? (float*)(ws + p.part_off) : nullptr;
   if ((p.dz || p.part) && a.rows > 0) {
-    T* to = p.dz ? (T*)(ws + p.dz_off) : nullptr;
+    const int vec = a.out_features % 8 == 0 && aligned16(a.g_out) && a.ld_g_out * E % 16 == 0 && (a.act == SGA_ACT_NONE || aligned16(a.pre));
     hipLaunchKernelGGL((token_dz_kernel<T>), dim3((unsigned)ceil_div(a.out_features, 256), (unsigned)p.chunks), dim3(256), 0, st, (const T*)a.g_out,
-                       a.ld_g_out, (const T*)a.pre, a.act, make_drop(a.dropout), to, part, a.rows, (int64_t)a.out_features, p.per);
+                       a.ld_g_out, (const T*)a.pre, a.act, make_drop(a.dropout), p.dz ? (T*)(ws + p.dz_off) : nullptr, p.ld_dz, part, a.rows,
+                       (int64_t)a.out_features, p.per, vec);
     LAUNCHED();
-    if (p.dz) { dz = to; ld_dz = a.out_features; }
   }
   if (p.part) {
     hipLaunchKernelGGL((token_sum_parts_kernel<T>), dim3((unsigned)ceil_div(a.out_features, 256)), dim3(256), 0, st, part, p.chunks, (T*)a.g_bias,
                        (int64_t)a.out_features);
     LAUNCHED();
   }
-  Epilogue e = {};
   if (a.g_x && a.rows > 0) {
-    e.out = a.g_x; e.ld_out = e.cols = a.in_features;
-    const int s = product<T>(dz, ld_dz, 1, a.w, 1, a.ld_w, a.rows, a.in_features, a.out_features, e, st);
+    const int s = launch_product(p.gx, ws + p.prod_off, st);
     if (s != SGA_OK) return s;
   }
-  if (a.g_w) {
-    e.out = a.g_w; e.ld_out = e.cols = a.in_features;
-    const int s = product<T>(dz, 1, ld_dz, a.x, 1, a.ld_x, a.out_features, a.in_features, a.rows, e, st);
-    if (s != SGA_OK) return s;
-  }
-  return SGA_OK;
+  return a.g_w ? launch_product(p.gw, ws + p.prod_off, st) : SGA_OK;
 }
 
 }  // namespace
@@ -192,22 +194,23 @@ int sga_op_linear_workspace(const sga_linear* a, int backward, int64_t* bytes) {
   if (!bytes) return SGA_ERR_BAD_ARG;
   const int st = backward ? bwd_check(a) : fwd_check(a);
   if (st != SGA_OK) return st;
-  *bytes = backward ? bwd_plan(*a).bytes : 0;
+  *bytes = backward ? bwd_plan(*a, nullptr).bytes : a->rows > 0 ? product_workspace(forward_product(*a)) : 0;
   return SGA_OK;
 }
 
 int sga_op_linear_fwd(const sga_linear* a, void* workspace, int64_t workspace_bytes, void* stream) {
   const int st = fwd_check(a);
   if (st != SGA_OK || a->rows == 0) return st;
-  hipStream_t s = (hipStream_t)stream;
-  (void)workspace; (void)workspace_bytes;
-  return a->dtype == SGA_DTYPE_F32 ? linear_fwd<float>(*a, s) : a->dtype == SGA_DTYPE_BF16 ? linear_fwd<bf16>(*a, s) : linear_fwd<f16>(*a, s);
+  const Product p = forward_product(*a);
+  const int64_t need = product_workspace(p);
+  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))) return SGA_ERR_BAD_ARG;
+  return launch_product(p, (char*)workspace, (hipStream_t)stream);
 }
 
 int sga_op_linear_bwd(const sga_linear* a, void* workspace, int64_t workspace_bytes, void* stream) {
   const int st = bwd_check(a);
   if (st != SGA_OK) return st;
-  const int64_t need = bwd_plan(*a).bytes;
+  const int64_t need = bwd_plan(*a, nullptr).bytes;
   if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))) return SGA_ERR_BAD_ARG;
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;

@@ -1,0 +1,410 @@
+// C[m, n] = epilogue(sum_k X(m, k) W(n, k)): the matrix product of the token blocks on the CDNA4 matrix pipe.
+//
+// A workgroup owns a BM x BN tile.  K is walked in steps of 128 bytes per row (64 elements of 16 bits, 32 of 32 bits); a step's
+// two operand tiles are moved by LDS-DMA (buffer_load_dwordx4 ... lds: 16 bytes per lane, no registers in between) into one of
+// two LDS stages while the other is multiplied.  Both memory orders of an operand are read as they lie:
+//   K adjacent  LDS rows of 128 bytes, one per m (n); a lane's fragment is one ds_read_b128
+//   K strided   LDS rows of BM (BN) elements, one per k; fragments by the transposing ds_read_b64_tr_b16 (16 bit) or
+//               ds_read_b32 (32 bit)
+// with the 16-byte pieces of a row permuted by the row index (the lanes of the DMA fetch permuted addresses: LDS-DMA writes lane
+// after lane), so that the fragment reads of a wave spread over all banks.  Rows past M or N repeat the last one (not stored),
+// pieces past K are out of the buffer descriptor's range and arrive as zeros.
+//
+// The product is taken as W X^T per wave (MFMA rows = n, columns = m): a lane then holds 4 adjacent n of one m.  Results pass
+// through LDS once more (32 rows of f32 per wave) so that every lane stores 8 adjacent columns, with bias, activation,
+// dropout words (two Philox calls for 8 columns), residual and the one rounding on the way.
+#include <type_traits>
+
+#include "token_common.h"
+
+using namespace token;
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char lds_char;
+
+struct TileArgs {
+  const char* x; const char* w;
+  int64_t ld_x, ld_w;            // bytes
+  int64_t M, N;
+  int64_t K;
+  int nk;                        // K steps
+  int ntm, ntn, nsplit;
+  float* part; int64_t ld_part;  // nsplit > 1: slab s of raw sums at part + s * M * ld_part
+  Epilogue e;
+};
+
+template <typename T> struct Frag;
+template <> struct Frag<bf16> {
+  typedef bf16 v8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Frag<f16> {
+  typedef f16 v8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Frag<float> {
+  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+    return c;
+  }
+};
+
+// 16 bytes per lane from buffer `srd` + voff into LDS at `lds` (wave-uniform) + lane * 16.  The wait is the caller's
+// (barrier_all): no register is written, so the compiler has nothing to track.
+__device__ __forceinline__ void dma16(uint32_t lds, uint32_t voff, i32x4 srd) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(srd) : "memory");      // m0 is reserved: the compiler sets it before any use of its own
+#endif
+}
+// everything this wave has in flight has landed, then all waves of the workgroup have got here
+__device__ __forceinline__ void barrier_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(lds_char*)p; }
+
+constexpr uint32_t kOutside = 0x80000000u;      // = num_records: a lane with this offset reads zeros
+
+// One operand's tile of R rows (m or n) per K step: how it is fetched and how its fragments are read
+template <typename T, int R, bool S, int NT>
+struct Side {
+  static constexpr int E = sizeof(T), KS = 128 / E, PASSES = R * 8 / NT, CPR = R * E / 16;      // KS: k per step; CPR: pieces per k row
+  static_assert(R * 8 % NT == 0, "tile / threads");
+  const char* base;
+  int64_t step;
+  uint32_t voff[PASSES];
+  int kpos[PASSES];         // strided: k row of the piece; adjacent: its k offset in bytes (the same for all passes)
+
+  __device__ __forceinline__ void init(const char* p, int64_t ld, int64_t r0, int64_t rows, int kstep0) {
+    const int t = threadIdx.x;
+    if constexpr (!S) {
+      base = p + r0 * ld + (int64_t)kstep0 * 128;
+      step = 128;
+      const int chunk = (t & 7) ^ ((t >> 3) & 7);
+      const int64_t last = rows - 1 - r0;
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) {
+        int64_t row = (i * NT + t) >> 3;
+        row = row < last ? row : last;
+        voff[i] = (uint32_t)(row * ld + chunk * 16);
+        kpos[i] = chunk * 16;
+      }
+    } else {
+      base = p + r0 * E + (int64_t)kstep0 * KS * ld;
+      step = (int64_t)KS * ld;
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) {
+        const int idx = i * NT + t, krow = idx / CPR, slot = idx % CPR;
+        const int chunk = E == 2 ? slot ^ ((krow & 3) << 1) : slot;
+        voff[i] = (r0 * E + chunk * 16 < rows * E) ? (uint32_t)(krow * ld + chunk * 16) : kOutside;
+        kpos[i] = krow;
+      }
+    }
+  }
+  // fetch the next step's tile into LDS at `lds`; k_left: elements of K from this step's start on
+  __device__ __forceinline__ void fetch(uint32_t lds, int64_t k_left) {
+    const uint64_t b = (uint64_t)base;
+    i32x4 srd;
+    srd[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+    srd[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xffff);
+    srd[2] = (int)kOutside;
+    srd[3] = 0x00027000;
+    const uint32_t wl = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x & ~63u) * 16);
+    if (k_left >= KS) {
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) dma16(wl + i * NT * 16, voff[i], srd);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) {
+        const bool in = S ? kpos[i] < k_left : kpos[i] < k_left * E;
+        dma16(wl + i * NT * 16, in ? voff[i] : kOutside, srd);
+      }
+    }
+    base += step;
+  }
+  // fragment of the 32 rows from r on, k group kk (of 4): per lane 16 bytes = row (lane & 31), k = 16-byte piece 2 kk + (lane >> 5)
+  static __device__ __forceinline__ u32x4 frag(const char* tile, int r, int kk) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (!S) {
+      return *(const u32x4*)(tile + (r + (lane & 31)) * 128 + (((2 * kk + (lane >> 5)) ^ (lane & 7)) << 4));
+    } else if constexpr (E == 2) {
+      const int i = lane & 15, g = lane >> 4;
+      u32x4 v = {};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int krow = kk * 16 + (g >> 1) * 8 + h * 4 + (i >> 2);
+        const int chunk = (r >> 3) + (g & 1) * 2 + ((i & 3) >> 1);
+        const char* p = tile + krow * (R * E) + ((chunk ^ ((krow & 3) << 1)) << 4) + (i & 1) * 8;
+#if defined(__HIP_DEVICE_COMPILE__)
+        const s16x4 q = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+        const unsigned long long u = __builtin_bit_cast(unsigned long long, q);
+        v[2 * h] = (unsigned)u;
+        v[2 * h + 1] = (unsigned)(u >> 32);
+#endif
+      }
+      return v;
+    } else {
+      u32x4 v = {};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = *(const uint32_t*)(tile + (kk * 8 + (lane >> 5) * 4 + j) * (R * E) + (r + (lane & 31)) * 4);
+      return v;
+    }
+  }
+};
+
+template <typename T, int TM, int TN, int WM, int WN, bool XS, bool WS>
+__global__ __launch_bounds__(WM * WN * 64, 1) void token_tile_kernel(const TileArgs a) {
+  constexpr int NT = WM * WN * 64, BM = WM * TM * 32, BN = WN * TN * 32, STAGE = (BM + BN) * 128;
+  constexpr int PITCH = TN * 32 + 4;
+  typedef Side<T, BM, XS, NT> X;
+  typedef Side<T, BN, WS, NT> W;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+
+  // Blocks go to the 8 XCDs in turn; each XCD gets a contiguous run of tiles, walked in bands of 8 tile rows: the ~32 tiles that
+  // are in flight on it form a patch whose operand rows its L2 holds
+  const int tiles = a.ntm * a.ntn, nb = tiles * a.nsplit;
+  const int xcd = blockIdx.x & 7, q = nb >> 3, rem = nb & 7;
+  const int t = xcd * q + (xcd < rem ? xcd : rem) + (blockIdx.x >> 3);
+  const int z = t / tiles, tile = t - z * tiles;
+  const int band = tile / (8 * a.ntn), in = tile - band * 8 * a.ntn, bm = a.ntm - band * 8 < 8 ? a.ntm - band * 8 : 8;
+  const int64_t m0 = (int64_t)(band * 8 + in % bm) * BM, n0 = (int64_t)(in / bm) * BN;
+  const int k0 = (int)((int64_t)a.nk * z / a.nsplit), k1 = (int)((int64_t)a.nk * (z + 1) / a.nsplit);
+
+  X sx;
+  W sw;
+  sx.init(a.x, a.ld_x, m0, a.M, k0);
+  sw.init(a.w, a.ld_w, n0, a.N, k0);
+  const uint32_t l0 = lds_addr(smem);
+  int64_t k_left = a.K - (int64_t)k0 * X::KS;
+  auto fetch = [&](int stage) {
+    sx.fetch(l0 + stage * STAGE, k_left);
+    sw.fetch(l0 + stage * STAGE + BM * 128, k_left);
+    k_left -= X::KS;
+  };
+  const int wave = threadIdx.x >> 6, wm = (wave % WM) * TM * 32, wn = (wave / WM) * TN * 32;
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int c = 0; c < 16; ++c) acc[i][j][c] = 0.f;
+  u32x4 fx[2][TM], fw[2][TN];
+  auto read = [&](int set, int stage, int kk) {
+    const char* s = smem + stage * STAGE;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) fx[set][i] = X::frag(s, wm + i * 32, kk);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) fw[set][j] = W::frag(s + BM * 128, wn + j * 32, kk);
+  };
+  auto mma = [&](int set) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = Frag<T>::mma(fw[set][j], fx[set][i], acc[i][j]);
+  };
+
+  // The last quarter of a step is multiplied after the barrier that ends it: its fragments are in registers, and the reads of the
+  // next stage's first quarter, which only now may start, pass under those products.
+  if (k1 > k0) {
+    fetch(0);
+    barrier_all();
+    if (k1 - k0 > 1) fetch(1);
+    read(0, 0, 0);
+    int stage = 0;
+    for (int k = k0; k < k1; ++k) {
+      read(1, stage, 1);
+      mma(0);
+      read(0, stage, 2);
+      mma(1);
+      read(1, stage, 3);
+      mma(0);
+      barrier_all();
+      if (k + 1 < k1) read(0, stage ^ 1, 0);
+      if (k + 2 < k1) fetch(stage);
+      mma(1);
+      stage ^= 1;
+    }
+  }
+
+  float* sh = (float*)smem + wave * (32 * PITCH);
+  const int lane = threadIdx.x & 63;
+  uint64_t seed = 0, offset = 0;
+  if (a.e.drop.on) drop_key(a.e.drop, seed, offset);
+  constexpr int LPR = TN * 4, RPP = 64 / LPR;      // lanes per row of 8-column pieces, rows per pass
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *(f32x4*)(sh + (lane & 31) * PITCH + j * 32 + c * 8 + (lane >> 5) * 4) =
+            f32x4{acc[i][j][c * 4], acc[i][j][c * 4 + 1], acc[i][j][c * 4 + 2], acc[i][j][c * 4 + 3]};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the rows below are other lanes' writes of this wave
+#pragma unroll 1
+    for (int r = lane / LPR; r < 32; r += RPP) {
+      float v[8];
+      load8(sh + r * PITCH + (lane % LPR) * 8, v);
+      const int64_t m = m0 + wm + i * 32 + r, n = n0 + wn + (lane % LPR) * 8;
+      if (m >= a.M || n >= a.N) continue;
+      if (a.nsplit > 1) store8(a.part + ((int64_t)z * a.M + m) * a.ld_part + n, v);
+      else epilogue8<T>(a.e, seed, offset, m, n, v);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+
+// out = epilogue(sum of the slabs, in their order)
+template <typename T>
+__global__ __launch_bounds__(256) void token_join_kernel(const float* __restrict__ part, int nsplit, int64_t M, int64_t ld_part, const Epilogue e) {
+  const int64_t per = ld_part / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= M * per) return;
+  const int64_t m = i / per, n = (i - m * per) * 8;
+  uint64_t seed = 0, offset = 0;
+  if (e.drop.on) drop_key(e.drop, seed, offset);
+  float v[8], u[8];
+  load8(part + m * ld_part + n, v);
+  for (int s = 1; s < nsplit; ++s) {
+    load8(part + ((int64_t)s * M + m) * ld_part + n, u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += u[j];
+  }
+  epilogue8<T>(e, seed, offset, m, n, v);
+}
+
+// dst [rows][cols_pad] = src [rows][cols], zeros behind: an operand whose rows are not 16-byte pieces
+template <typename U>
+__global__ __launch_bounds__(256) void token_pack_kernel(const U* __restrict__ src, int64_t ld, U* __restrict__ dst, int64_t rows, int cols, int cols_pad) {
+  constexpr int V = 16 / sizeof(U);
+  typedef U v16 __attribute__((ext_vector_type(V)));
+  const int per = cols_pad / V;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per;
+    const int c = (int)(i - r * per) * V;
+    v16 v;
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = c + j < cols ? src[r * ld + c + j] : (U)0;
+    *(v16*)(dst + r * cols_pad + c) = v;
+  }
+}
+
+#define LAUNCHED() do { if (hipGetLastError() != hipSuccess) return SGA_ERR_HIP; } while (0)
+
+// How a product is run
+struct Plan {
+  int tile;                  // index into the tile table
+  int nsplit;
+  bool pack_x, pack_w;
+  int64_t ldp_x, ldp_w;      // elements, packed
+  int64_t x_off, w_off, part_off, bytes, ld_part;
+};
+
+bool needs_pack(const Operand& o, int64_t rows, int64_t K, int E) {
+  const int64_t inner = o.strided ? rows : K, outer = o.strided ? 128 / E : 256;
+  // 16-byte pieces all along, and a tile's rows within the 2 GiB that an offset of the buffer descriptor spans
+  return ((uintptr_t)o.p & 15) || (o.ld * E) % 16 || (!o.padded && (inner * E) % 16) || outer * o.ld * E >= (1ll << 31) - 65536;
+}
+
+constexpr int kTiles = 3;
+const int kTileM[kTiles] = {256, 128, 64}, kTileN[kTiles] = {256, 128, 64};
+
+Plan make_plan(const Product& p) {
+  const int E = (int)dtype_bytes(p.dtype), V = 16 / E;
+  Plan o = {};
+  o.pack_x = needs_pack(p.x, p.M, p.K, E);
+  o.pack_w = needs_pack(p.w, p.N, p.K, E);
+  if (o.pack_x) { o.ldp_x = round_up(p.x.strided ? p.M : p.K, V); o.x_off = o.bytes; o.bytes += round_up((p.x.strided ? p.K : p.M) * o.ldp_x * E, 256); }
+  if (o.pack_w) { o.ldp_w = round_up(p.w.strided ? p.N : p.K, V); o.w_off = o.bytes; o.bytes += round_up((p.w.strided ? p.K : p.N) * o.ldp_w * E, 256); }
+  const int64_t nk = ceil_div(p.K, 128 / E);
+  double best = 1e300;
+  o.nsplit = 1;
+  for (int t = 0; t < kTiles; ++t) {
+    const int64_t tiles = ceil_div(p.M, kTileM[t]) * ceil_div(p.N, kTileN[t]);
+    static const int slots[kTiles] = {256, 512, 1024};
+    static const double per_step[kTiles] = {1.0, 0.62, 0.34};      // time of a K step of one workgroup with its CU shared by the others, relative
+    for (int s = 1; s == 1 || (s <= 16 && s <= nk); s *= 2) {
+      const double rounds = (double)ceil_div(tiles * s, slots[t]);
+      double cost = rounds * ((double)ceil_div(nk, s) + 4.0) * per_step[t];
+      if (s > 1) cost += 4.0 + (double)p.M * p.N * s * 8.0 / 4e12 / 0.9e-6;
+      if (cost < best) { best = cost; o.tile = t; o.nsplit = s; }
+    }
+  }
+  if (o.nsplit > 1) { o.ld_part = round_up(p.N, 8); o.part_off = o.bytes; o.bytes += round_up(o.nsplit * p.M * o.ld_part * 4, 256); }
+  return o;
+}
+
+template <typename T, int TM, int TN, int WM, int WN, bool XS, bool WS>
+int run_tile(const TileArgs& a, hipStream_t st) {
+  constexpr int BM = WM * TM * 32, BN = WN * TN * 32, MAIN = 2 * (BM + BN) * 128, EPI = WM * WN * 32 * (TN * 32 + 4) * 4;
+  constexpr int LDS = MAIN > EPI ? MAIN : EPI;
+  const void* f = reinterpret_cast<const void*>(&token_tile_kernel<T, TM, TN, WM, WN, XS, WS>);
+  if (LDS > 65536 && hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return SGA_ERR_HIP;
+  hipLaunchKernelGGL((token_tile_kernel<T, TM, TN, WM, WN, XS, WS>), dim3((unsigned)(a.ntm * a.ntn * a.nsplit)), dim3(WM * WN * 64), LDS, st, a);
+  LAUNCHED();
+  return SGA_OK;
+}
+template <typename T, bool XS, bool WS>
+int run_tile_of(int tile, const TileArgs& a, hipStream_t st) {
+  switch (tile) {
+    case 0: return run_tile<T, 4, 2, 2, 4, XS, WS>(a, st);
+    case 1: return run_tile<T, 2, 2, 2, 2, XS, WS>(a, st);
+    default: return run_tile<T, 1, 1, 2, 2, XS, WS>(a, st);
+  }
+}
+
+template <typename T>
+int run(const Product& p, char* ws, hipStream_t st) {
+  const Plan o = make_plan(p);
+  TileArgs a = {};
+  typedef typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type U;
+  auto side = [&](const Operand& op, int64_t rows, bool pack, int64_t ldp, int64_t off, const char*& q, int64_t& ld) -> int {
+    q = (const char*)op.p;
+    ld = op.ld * (int64_t)sizeof(T);
+    if (!pack) return SGA_OK;
+    const int64_t outer = op.strided ? p.K : rows, inner = op.strided ? rows : p.K;
+    const int64_t blocks = ceil_div(outer * ldp / (16 / (int)sizeof(U)), 256);
+    hipLaunchKernelGGL((token_pack_kernel<U>), dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, st, (const U*)op.p, op.ld, (U*)(ws + off),
+                       outer, (int)inner, (int)ldp);
+    LAUNCHED();
+    q = ws + off;
+    ld = ldp * (int64_t)sizeof(T);
+    return SGA_OK;
+  };
+  int s = side(p.x, p.M, o.pack_x, o.ldp_x, o.x_off, a.x, a.ld_x);
+  if (s == SGA_OK) s = side(p.w, p.N, o.pack_w, o.ldp_w, o.w_off, a.w, a.ld_w);
+  if (s != SGA_OK) return s;
+  a.M = p.M; a.N = p.N; a.K = p.K;
+  a.nk = (int)ceil_div(p.K, 128 / (int)sizeof(T));
+  a.ntm = (int)ceil_div(p.M, kTileM[o.tile]);
+  a.ntn = (int)ceil_div(p.N, kTileN[o.tile]);
+  a.nsplit = o.nsplit;
+  a.part = o.nsplit > 1 ? (float*)(ws + o.part_off) : nullptr;
+  a.ld_part = o.ld_part;
+  a.e = p.e;
+  if ((int64_t)a.ntm * a.ntn * a.nsplit > 0x7fffffff) return SGA_ERR_UNSUPPORTED;
+  if (!p.x.strided && !p.w.strided) s = run_tile_of<T, false, false>(o.tile, a, st);
+  else if (!p.x.strided) s = run_tile_of<T, false, true>(o.tile, a, st);
+  else s = run_tile_of<T, true, true>(o.tile, a, st);
+  if (s != SGA_OK || o.nsplit == 1) return s;
+  hipLaunchKernelGGL((token_join_kernel<T>), dim3((unsigned)ceil_div(p.M * (o.ld_part / 8), 256)), dim3(256), 0, st, a.part, o.nsplit, p.M, o.ld_part, p.e);
+  LAUNCHED();
+  return SGA_OK;
+}
+
+}  // namespace
+
+namespace token {
+
+int64_t product_workspace(const Product& p) { return make_plan(p).bytes; }
+
+int launch_product(const Product& p, char* ws, hipStream_t st) {
+  return p.dtype == SGA_DTYPE_F32 ? run<float>(p, ws, st) : p.dtype == SGA_DTYPE_BF16 ? run<bf16>(p, ws, st) : run<f16>(p, ws, st);
+}
+
+}  // namespace token
