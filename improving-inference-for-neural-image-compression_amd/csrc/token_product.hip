@@ -260,6 +260,105 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void token_tile_kernel(const TileA
   }
 }
 
+// ---- few rows of X (tokens of as many sequences): the weight's rows are read once, straight into fragments ------------------
+// A workgroup of 8 waves owns 16 columns n.  The waves share out K in pieces of 128 bytes per row of w, so that a wave reads whole
+// lines; MFMA rows = the 16 columns, MFMA columns = 16 rows of X (MB of them).  Any order of k inside a piece serves, as both
+// operands take the same: lane (r, q) takes bytes q * 16 .. of each 64.  The waves' sums meet in LDS.
+template <typename T> struct Frag16;
+template <> struct Frag16<bf16> {
+  typedef bf16 v8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Frag16<f16> {
+  typedef f16 v8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Frag16<float> {
+  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+    return c;
+  }
+};
+
+struct FewArgs {
+  const char* x; const char* w;
+  int64_t ld_x, ld_w;            // bytes
+  int64_t M, N;
+  int kb;                        // bytes of a row
+  Epilogue e;
+};
+
+// 16 bytes of a row at byte b; zeros past its end.  VEC: rows are whole 16-byte pieces, aligned
+template <typename T, bool VEC>
+__device__ __forceinline__ u32x4 row_piece(const char* row, int b, int kb) {
+  u32x4 v = {0, 0, 0, 0};
+  if constexpr (VEC) {
+    if (b < kb) v = *(const u32x4*)(row + b);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) if (b + 4 * j < kb) v[j] = *(const uint32_t*)(row + b + 4 * j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (b + 2 * j < kb) v[j >> 1] |= (uint32_t)*(const uint16_t*)(row + b + 2 * j) << (16 * (j & 1));
+  }
+  return v;
+}
+
+template <typename T, int MB, bool VEC>
+__global__ __launch_bounds__(512, 1) void token_few_kernel(const FewArgs a) {
+  __shared__ __attribute__((aligned(16))) float sh[8][MB * 16][20];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const char* wrow = a.w + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ld_w;
+  const char* xrow[MB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i) xrow[i] = a.x + (i * 16 + r < a.M ? i * 16 + r : a.M - 1) * a.ld_x;
+  f32x4 acc[MB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  constexpr int U = VEC ? (MB == 1 ? 4 : 2) : 1;      // pieces in flight
+  for (int b0 = wave * 128; b0 < a.kb; b0 += 1024 * U) {
+    u32x4 fw[U][2], fx[U][2][MB];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int b = b0 + u * 1024 + h * 64 + q * 16;
+        fw[u][h] = row_piece<T, VEC>(wrow, b, a.kb);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) fx[u][h][i] = row_piece<T, VEC>(xrow[i], b, a.kb);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < MB; ++i) acc[i] = Frag16<T>::mma(fw[u][h], fx[u][h][i], acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < MB; ++i) *(f32x4*)&sh[wave][i * 16 + r][q * 4] = acc[i];
+  __syncthreads();
+  const int m = threadIdx.x >> 1, c = (threadIdx.x & 1) * 8;
+  if (m >= a.M || n0 + c >= a.N) return;
+  float v[8], u[8];
+  load8(&sh[0][m][c], v);
+#pragma unroll
+  for (int s = 1; s < 8; ++s) {
+    load8(&sh[s][m][c], u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += u[j];
+  }
+  uint64_t seed = 0, offset = 0;
+  if (a.e.drop.on) drop_key(a.e.drop, seed, offset);
+  epilogue8<T>(a.e, seed, offset, m, n0 + c, v);
+}
+
 // out = epilogue(sum of the slabs, in their order)
 template <typename T>
 __global__ __launch_bounds__(256) void token_join_kernel(const float* __restrict__ part, int nsplit, int64_t M, int64_t ld_part, const Epilogue e) {
@@ -298,6 +397,7 @@ __global__ __launch_bounds__(256) void token_pack_kernel(const U* __restrict__ s
 
 // How a product is run
 struct Plan {
+  int few;                   // 16-row blocks of token_few_kernel, 0: tiles
   int tile;                  // index into the tile table
   int nsplit;
   bool pack_x, pack_w;
@@ -311,12 +411,17 @@ bool needs_pack(const Operand& o, int64_t rows, int64_t K, int E) {
   return ((uintptr_t)o.p & 15) || (o.ld * E) % 16 || (!o.padded && (inner * E) % 16) || outer * o.ld * E >= (1ll << 31) - 65536;
 }
 
+constexpr int64_t kFewRows = 64;
 constexpr int kTiles = 3;
 const int kTileM[kTiles] = {256, 128, 64}, kTileN[kTiles] = {256, 128, 64};
 
 Plan make_plan(const Product& p) {
   const int E = (int)dtype_bytes(p.dtype), V = 16 / E;
   Plan o = {};
+  if (!p.x.strided && !p.w.strided && p.M <= kFewRows) {
+    o.few = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
+    return o;
+  }
   o.pack_x = needs_pack(p.x, p.M, p.K, E);
   o.pack_w = needs_pack(p.w, p.N, p.K, E);
   if (o.pack_x) { o.ldp_x = round_up(p.x.strided ? p.M : p.K, V); o.x_off = o.bytes; o.bytes += round_up((p.x.strided ? p.K : p.M) * o.ldp_x * E, 256); }
@@ -358,9 +463,22 @@ int run_tile_of(int tile, const TileArgs& a, hipStream_t st) {
   }
 }
 
+template <typename T, int MB>
+int run_few(const Product& p, hipStream_t st) {
+  const int64_t E = sizeof(T);
+  const FewArgs a = {(const char*)p.x.p, (const char*)p.w.p, p.x.ld * E, p.w.ld * E, p.M, p.N, (int)(p.K * E), p.e};
+  const bool vec = !(((uintptr_t)a.x | (uintptr_t)a.w | (uint64_t)a.ld_x | (uint64_t)a.ld_w | (uint64_t)a.kb) & 15);
+  const dim3 grid((unsigned)ceil_div(p.N, 16));
+  if (vec) hipLaunchKernelGGL((token_few_kernel<T, MB, true>), grid, dim3(512), 0, st, a);
+  else hipLaunchKernelGGL((token_few_kernel<T, MB, false>), grid, dim3(512), 0, st, a);
+  LAUNCHED();
+  return SGA_OK;
+}
+
 template <typename T>
 int run(const Product& p, char* ws, hipStream_t st) {
   const Plan o = make_plan(p);
+  if (o.few) return o.few == 1 ? run_few<T, 1>(p, st) : o.few == 2 ? run_few<T, 2>(p, st) : run_few<T, 4>(p, st);
   TileArgs a = {};
   typedef typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type U;
   auto side = [&](const Operand& op, int64_t rows, bool pack, int64_t ldp, int64_t off, const char*& q, int64_t& ld) -> int {
