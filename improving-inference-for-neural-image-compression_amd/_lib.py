@@ -210,6 +210,8 @@ class _CallLog:
             return str(v)
         if isinstance(v, float):
             return repr(v)
+        if isinstance(v, bytes) and 0 in v:      # an argument structure
+            return "P"
         if isinstance(v, bytes):
             return "S:" + v.decode(errors="replace").replace(" ", "_")
         if v is None:

@@ -22,6 +22,7 @@ There is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -30,11 +31,31 @@ from . import _lib
 ACTIVATIONS = tuple(_lib.ACTS)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _U64 = (1 << 64) - 1
-_byref = C.byref
+_Tensor = torch.Tensor
+_empty = torch.empty
+
+# The argument structures as bytes: a call is a few microseconds long, and filling a ctypes structure would be half of it.
+_DROP = "dQQP"
+_LINEAR = struct.Struct("@q4i PqPqPPqPqP Pq PPP " + _DROP).pack
+_NORM = struct.Struct("@q3if PqPP PPP PqPq PPP").pack
+_DROPOUT = struct.Struct("@" + _DROP).pack
+_NO_DROP = (0.0, 0, 0, 0)
+_NOMEM = -6
+_entry = {}
 
 
 def _rows(t, what, dtype=None, device=None, features=None):
     """-> (rows, features, row stride) of a tensor whose leading dimensions collapse into one."""
+    if isinstance(t, _Tensor) and t.is_cuda and t.is_contiguous() and (device is None or t.device == device):
+        shape = t.shape
+        if (t.dtype is dtype if dtype is not None else t.dtype in _DTYPES) and len(shape) and shape[-1]:
+            n = shape[-1]
+            if features is None or n == features:
+                return t.numel() // n, n, n
+    return _rows_of_any(t, what, dtype, device, features)
+
+
+def _rows_of_any(t, what, dtype, device, features):
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s: a tensor is expected, got %s" % (what, type(t).__name__))
     if t.dtype not in _DTYPES or (dtype is not None and t.dtype != dtype):
@@ -65,7 +86,7 @@ def _rows(t, what, dtype=None, device=None, features=None):
 
 def _vector(t, what, n, dtypes, device):
     if t is None:
-        return None
+        return 0
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
         raise TypeError("%s: a tensor of %s is expected" % (what, " or ".join(str(d) for d in dtypes)))
     if t.device != device or tuple(t.shape) != (n,) or not t.is_contiguous():
@@ -74,7 +95,7 @@ def _vector(t, what, n, dtypes, device):
 
 
 def _same(t, like, what):
-    if tuple(t.shape) != tuple(like):
+    if t.shape != like:
         raise ValueError("%s has shape %s, %s is expected" % (what, tuple(t.shape), tuple(like)))
 
 
@@ -85,19 +106,20 @@ def _contiguous(t, what):
 
 
 def _drop(dropout, device):
+    """-> the members of sga_dropout"""
     if dropout is None:
-        return _lib.SgaDropout()
+        return _NO_DROP
     p = float(dropout[0])
     if not 0.0 <= p <= 1.0:
         raise ValueError("dropout: a probability is expected, got %r" % (dropout[0],))
-    if len(dropout) == 2 and isinstance(dropout[1], torch.Tensor):
+    if len(dropout) == 2 and isinstance(dropout[1], _Tensor):
         s = dropout[1]
         if s.dtype != torch.int64 or s.numel() != 2 or not s.is_contiguous() or s.device != device:
             raise ValueError("dropout: the state is an int64 tensor {seed, offset} on %s" % device)
-        return _lib.SgaDropout(p, 0, 0, s.data_ptr())
+        return p, 0, 0, s.data_ptr()
     if len(dropout) != 3:
         raise ValueError("dropout: (p, seed, offset) or (p, state tensor) is expected")
-    return _lib.SgaDropout(p, int(dropout[1]) & _U64, int(dropout[2]) & _U64, None)
+    return p, int(dropout[1]) & _U64, int(dropout[2]) & _U64, 0
 
 
 def _act(act):
@@ -107,21 +129,30 @@ def _act(act):
         raise ValueError("act: one of %s is expected, got %r" % (", ".join(ACTIVATIONS), act)) from None
 
 
-def _call(name, a, device, backward=None):
-    """Runs entry point `name` on the arguments `a`; backward: None (no workspace) or which workspace is asked for."""
-    lib = _lib.load_library()
-    with torch.cuda.device(device):
-        stream = torch.cuda.current_stream(device).cuda_stream
-        if backward is None:
-            st = getattr(lib, name)(_byref(a), stream)
-        else:
-            need = C.c_int64(0)
-            st = getattr(lib, name.rsplit("_", 1)[0] + "_workspace")(_byref(a), backward, _byref(need))
-            if st == 0:
-                n = need.value
-                ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-                st = getattr(lib, name)(_byref(a), ws.data_ptr() if n else None, n, stream)
-    _lib.check(lib, None, st, name)
+def _call(name, device, *args):
+    """An entry point on the device's current stream -> status."""
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(_lib.load_library(), name)
+    i = device.index
+    if torch._C._cuda_getDevice() == i:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    with torch.cuda.device(i):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(i))
+
+
+def _call_with_workspace(name, a, device, backward):
+    """An entry point with the workspace that it asks for; a forward call is first made without one, which most need not have."""
+    st = _NOMEM if backward else _call(name, device, a, None, 0)
+    if st == _NOMEM:
+        need = C.c_int64(0)
+        st = getattr(_lib.load_library(), name[:-4] + "_workspace")(a, backward, C.addressof(need))
+        if st == 0:
+            n = need.value
+            ws = _empty(n, dtype=torch.uint8, device=device) if n else None
+            st = _call(name, device, a, ws.data_ptr() if n else None, n)
+    if st:
+        _lib.check(None, None, st, name)
 
 
 def linear(x, weight, bias=None, act="none", residual=None, dropout=None, want_pre=False, out=None):
@@ -135,20 +166,22 @@ def linear(x, weight, bias=None, act="none", residual=None, dropout=None, want_p
     if weight.dim() != 2:
         raise ValueError("weight: [out_features, in_features] is expected, got shape %s" % (tuple(weight.shape),))
     shape = x.shape[:-1] + (n,)
-    ld_res = ld_out = n
+    ld_res, ld_out, p_res, p_pre, pre = n, n, 0, 0, None
     if residual is not None:
         _, _, ld_res = _rows(residual, "residual", dt, dev, n)
         _same(residual, shape, "residual")
+        p_res = residual.data_ptr()
     if out is None:
-        out = torch.empty(shape, dtype=dt, device=dev)
+        out = _empty(shape, dtype=dt, device=dev)
     else:
         _, _, ld_out = _rows(out, "out", dt, dev, n)
         _same(out, shape, "out")
-    pre = torch.empty(shape, dtype=dt, device=dev) if want_pre else None
-    a = _lib.SgaLinear(rows, k, n, _DTYPES[dt], _act(act), x.data_ptr(), ld_x, weight.data_ptr(), ld_w,
-                       _vector(bias, "bias", n, (dt,), dev), residual.data_ptr() if residual is not None else None, ld_res,
-                       out.data_ptr(), ld_out, pre.data_ptr() if want_pre else None, None, 0, None, None, None, _drop(dropout, dev))
-    _call("sga_op_linear_fwd", a, dev, 0)
+    if want_pre:
+        pre = _empty(shape, dtype=dt, device=dev)
+        p_pre = pre.data_ptr()
+    a = _LINEAR(rows, k, n, _DTYPES[dt], _act(act), x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _vector(bias, "bias", n, (dt,), dev), p_res, ld_res,
+                out.data_ptr(), ld_out, p_pre, 0, 0, 0, 0, 0, *_drop(dropout, dev))
+    _call_with_workspace("sga_op_linear_fwd", a, dev, 0)
     return (out, pre) if want_pre else out
 
 
@@ -168,13 +201,13 @@ def linear_grad(g_out, x, weight, pre=None, act="none", dropout=None, want=(True
         _rows(pre, "pre", dt, dev, n)
         _same(pre, g_out.shape, "pre")
         _contiguous(pre, "pre")
-    g_x = torch.empty(x.shape, dtype=dt, device=dev) if want[0] else None
-    g_w = torch.empty((n, k), dtype=dt, device=dev) if want[1] else None
-    g_b = torch.empty(n, dtype=dt, device=dev) if want[2] else None
-    a = _lib.SgaLinear(rows, k, n, _DTYPES[dt], code, x.data_ptr(), ld_x, weight.data_ptr(), ld_w, None, None, 0, None, 0,
-                       pre.data_ptr() if code else None, g_out.data_ptr(), ld_g, g_x.data_ptr() if want[0] else None,
-                       g_w.data_ptr() if want[1] else None, g_b.data_ptr() if want[2] else None, _drop(dropout, dev))
-    _call("sga_op_linear_bwd", a, dev, 1)
+    g_x = _empty(x.shape, dtype=dt, device=dev) if want[0] else None
+    g_w = _empty((n, k), dtype=dt, device=dev) if want[1] else None
+    g_b = _empty(n, dtype=dt, device=dev) if want[2] else None
+    a = _LINEAR(rows, k, n, _DTYPES[dt], code, x.data_ptr(), ld_x, weight.data_ptr(), ld_w, 0, 0, 0, 0, 0, pre.data_ptr() if code else 0,
+                g_out.data_ptr(), ld_g, g_x.data_ptr() if want[0] else 0, g_w.data_ptr() if want[1] else 0, g_b.data_ptr() if want[2] else 0,
+                *_drop(dropout, dev))
+    _call_with_workspace("sga_op_linear_bwd", a, dev, 1)
     return g_x, g_w, g_b
 
 
@@ -188,12 +221,15 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, want_stats=False):
     w, b = _vector(weight, "weight", n, (dt, torch.float32), dev), _vector(bias, "bias", n, (pt,), dev)
     if not eps >= 0.0:
         raise ValueError("eps: a number >= 0 is expected, got %r" % (eps,))
-    y = torch.empty(x.shape, dtype=dt, device=dev)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev) if want_stats else None
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev) if want_stats else None
-    a = _lib.SgaLayerNorm(rows, n, _DTYPES[dt], _DTYPES[pt], eps, x.data_ptr(), ld, w, b, y.data_ptr(),
-                          mean.data_ptr() if want_stats else None, rstd.data_ptr() if want_stats else None)
-    _call("sga_op_layer_norm_fwd", a, dev)
+    y = _empty(x.shape, dtype=dt, device=dev)
+    p_mean = p_rstd = 0
+    if want_stats:
+        mean, rstd = _empty(x.shape[:-1], dtype=torch.float32, device=dev), _empty(x.shape[:-1], dtype=torch.float32, device=dev)
+        p_mean, p_rstd = mean.data_ptr(), rstd.data_ptr()
+    st = _call("sga_op_layer_norm_fwd", dev, _NORM(rows, n, _DTYPES[dt], _DTYPES[pt], eps, x.data_ptr(), ld, w, b, y.data_ptr(), p_mean, p_rstd,
+                                                   0, 0, 0, 0, 0, 0, 0))
+    if st:
+        _lib.check(None, None, st, "sga_op_layer_norm_fwd")
     return (y, mean, rstd) if want_stats else y
 
 
@@ -216,13 +252,13 @@ def layer_norm_grad(g_y, x, mean, rstd, weight=None, g_add=None, want=(True, Tru
     pt = weight.dtype if weight is not None else param_dtype or dt
     if pt not in (dt, torch.float32):
         raise TypeError("param_dtype: %s or torch.float32 is expected, got %s" % (dt, pt))
-    g_x = torch.empty(x.shape, dtype=dt, device=dev) if want[0] else None
-    g_w = torch.empty(n, dtype=pt, device=dev) if want[1] else None
-    g_b = torch.empty(n, dtype=pt, device=dev) if want[2] else None
-    a = _lib.SgaLayerNorm(rows, n, _DTYPES[dt], _DTYPES[pt], 0.0, x.data_ptr(), ld, w, None, None, mean.data_ptr(), rstd.data_ptr(),
-                          g_y.data_ptr(), ld_g, g_add.data_ptr() if g_add is not None else None, ld_add,
-                          g_x.data_ptr() if want[0] else None, g_w.data_ptr() if want[1] else None, g_b.data_ptr() if want[2] else None)
-    _call("sga_op_layer_norm_bwd", a, dev, 1)
+    g_x = _empty(x.shape, dtype=dt, device=dev) if want[0] else None
+    g_w = _empty(n, dtype=pt, device=dev) if want[1] else None
+    g_b = _empty(n, dtype=pt, device=dev) if want[2] else None
+    a = _NORM(rows, n, _DTYPES[dt], _DTYPES[pt], 0.0, x.data_ptr(), ld, w, 0, 0, mean.data_ptr(), rstd.data_ptr(), g_y.data_ptr(), ld_g,
+              g_add.data_ptr() if g_add is not None else 0, ld_add, g_x.data_ptr() if want[0] else 0, g_w.data_ptr() if want[1] else 0,
+              g_b.data_ptr() if want[2] else 0)
+    _call_with_workspace("sga_op_layer_norm_bwd", a, dev, 1)
     return g_x, g_w, g_b
 
 
@@ -235,11 +271,10 @@ def dropout(x, p, seed, offset=0, residual=None):
     if residual is not None:
         _, _, ld_res = _rows(residual, "residual", dt, dev, n)
         _same(residual, x.shape, "residual")
-    d = _drop((p, seed) if isinstance(seed, torch.Tensor) else (p, seed, offset), dev)
-    y = torch.empty(x.shape, dtype=dt, device=dev)
-    lib = _lib.load_library()
-    with torch.cuda.device(dev):
-        st = lib.sga_op_dropout(x.data_ptr(), ld, residual.data_ptr() if residual is not None else None, ld_res, y.data_ptr(), rows, n,
-                                _DTYPES[dt], _byref(d), torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(lib, None, st, "sga_op_dropout")
+    d = _DROPOUT(*_drop((p, seed) if isinstance(seed, _Tensor) else (p, seed, offset), dev))
+    y = _empty(x.shape, dtype=dt, device=dev)
+    st = _call("sga_op_dropout", dev, x.data_ptr(), ld, residual.data_ptr() if residual is not None else None, ld_res, y.data_ptr(), rows, n,
+               _DTYPES[dt], d)
+    if st:
+        _lib.check(None, None, st, "sga_op_dropout")
     return y

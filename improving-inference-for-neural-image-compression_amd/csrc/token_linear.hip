@@ -203,7 +203,7 @@ int sga_op_linear_fwd(const sga_linear* a, void* workspace, int64_t workspace_by
   if (st != SGA_OK || a->rows == 0) return st;
   const Product p = forward_product(*a);
   const int64_t need = product_workspace(p);
-  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))) return SGA_ERR_BAD_ARG;
+  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))) return SGA_ERR_NOMEM;
   return launch_product(p, (char*)workspace, (hipStream_t)stream);
 }
 
@@ -211,7 +211,7 @@ int sga_op_linear_bwd(const sga_linear* a, void* workspace, int64_t workspace_by
   const int st = bwd_check(a);
   if (st != SGA_OK) return st;
   const int64_t need = bwd_plan(*a, nullptr).bytes;
-  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))) return SGA_ERR_BAD_ARG;
+  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))) return SGA_ERR_NOMEM;
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;
   return a->dtype == SGA_DTYPE_F32 ? linear_bwd<float>(*a, ws, s) : a->dtype == SGA_DTYPE_BF16 ? linear_bwd<bf16>(*a, ws, s) : linear_bwd<f16>(*a, ws, s);

@@ -75,18 +75,33 @@ constexpr uint32_t kOutside = 0x80000000u;      // = num_records: a lane with th
 template <typename T, int R, bool S, int NT>
 struct Side {
   static constexpr int E = sizeof(T), KS = 128 / E, PASSES = R * 8 / NT, CPR = R * E / 16;      // KS: k per step; CPR: pieces per k row
-  static_assert(R * 8 % NT == 0, "tile / threads");
+  static_assert(R * 8 % NT == 0 && NT % 128 == 0, "tile / threads");
+  // Where piece `chunk` of row `row` lies in LDS, and back.  64 banks of 4 bytes serve 256 bytes a cycle; the lanes of one cycle
+  // read  adjacent: 16 rows at one chunk | strided, 16 bit: 4 k rows x 2 neighbouring pairs of chunks | strided, 32 bit: 2 k rows, 4
+  // apart, x 8 chunks.  These keys put them on different banks (a row of 128 bytes gives the first bit by itself).
+  static __device__ __forceinline__ int key(int row) {
+    if constexpr (!S) return (row >> 1) & 7;
+    else if constexpr (E == 4) return ((row >> 2) & 1) << 3;
+    else return R * E == 128 ? ((row >> 1) & 1) << 2 : (row & 3) << 1;
+  }
+  static constexpr bool FOLD = S && E == 2 && R * E > 128;      // the pair's lowest bit also goes into bit 3
+  static __device__ __forceinline__ int slot_of(int chunk, int row) { return chunk ^ key(row) ^ (FOLD ? (chunk & 2) << 2 : 0); }
+  static __device__ __forceinline__ int chunk_of(int slot, int row) {
+    const int c = slot ^ key(row);
+    return FOLD ? c ^ (c & 2) << 2 : c;
+  }
+
   const char* base;
   int64_t step;
   uint32_t voff[PASSES];
-  int kpos[PASSES];         // strided: k row of the piece; adjacent: its k offset in bytes (the same for all passes)
+  int kpos[PASSES];         // strided: k row of the piece; adjacent: its offset in bytes (the same for all passes)
 
   __device__ __forceinline__ void init(const char* p, int64_t ld, int64_t r0, int64_t rows, int kstep0) {
     const int t = threadIdx.x;
     if constexpr (!S) {
       base = p + r0 * ld + (int64_t)kstep0 * 128;
       step = 128;
-      const int chunk = (t & 7) ^ ((t >> 3) & 7);
+      const int chunk = chunk_of(t & 7, t >> 3);      // rows of one lane are NT / 8 apart: one key
       const int64_t last = rows - 1 - r0;
 #pragma unroll
       for (int i = 0; i < PASSES; ++i) {
@@ -101,38 +116,31 @@ struct Side {
 #pragma unroll
       for (int i = 0; i < PASSES; ++i) {
         const int idx = i * NT + t, krow = idx / CPR, slot = idx % CPR;
-        const int chunk = E == 2 ? slot ^ ((krow & 3) << 1) : slot;
+        const int chunk = chunk_of(slot, krow);
         voff[i] = (r0 * E + chunk * 16 < rows * E) ? (uint32_t)(krow * ld + chunk * 16) : kOutside;
         kpos[i] = krow;
       }
     }
   }
-  // fetch the next step's tile into LDS at `lds`; k_left: elements of K from this step's start on
-  __device__ __forceinline__ void fetch(uint32_t lds, int64_t k_left) {
+  // the next step's tile: open, then one piece after the other into LDS at `lds`; left: what of K there is from the step's start on, in
+  // bytes (adjacent) or rows (strided), 0 or less: nothing
+  i32x4 srd;
+  __device__ __forceinline__ void open() {
     const uint64_t b = (uint64_t)base;
-    i32x4 srd;
     srd[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
     srd[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xffff);
     srd[2] = (int)kOutside;
     srd[3] = 0x00027000;
-    const uint32_t wl = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x & ~63u) * 16);
-    if (k_left >= KS) {
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i) dma16(wl + i * NT * 16, voff[i], srd);
-    } else {
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i) {
-        const bool in = S ? kpos[i] < k_left : kpos[i] < k_left * E;
-        dma16(wl + i * NT * 16, in ? voff[i] : kOutside, srd);
-      }
-    }
     base += step;
+  }
+  __device__ __forceinline__ void piece(int i, uint32_t lds, int left) {
+    dma16(lds + i * NT * 16, kpos[i] < left ? voff[i] : kOutside, srd);
   }
   // fragment of the 32 rows from r on, k group kk (of 4): per lane 16 bytes = row (lane & 31), k = 16-byte piece 2 kk + (lane >> 5)
   static __device__ __forceinline__ u32x4 frag(const char* tile, int r, int kk) {
     const int lane = threadIdx.x & 63;
     if constexpr (!S) {
-      return *(const u32x4*)(tile + (r + (lane & 31)) * 128 + (((2 * kk + (lane >> 5)) ^ (lane & 7)) << 4));
+      return *(const u32x4*)(tile + (r + (lane & 31)) * 128 + (slot_of(2 * kk + (lane >> 5), lane & 31) << 4));
     } else if constexpr (E == 2) {
       const int i = lane & 15, g = lane >> 4;
       u32x4 v = {};
@@ -140,7 +148,7 @@ struct Side {
       for (int h = 0; h < 2; ++h) {
         const int krow = kk * 16 + (g >> 1) * 8 + h * 4 + (i >> 2);
         const int chunk = (r >> 3) + (g & 1) * 2 + ((i & 3) >> 1);
-        const char* p = tile + krow * (R * E) + ((chunk ^ ((krow & 3) << 1)) << 4) + (i & 1) * 8;
+        const char* p = tile + krow * (R * E) + (slot_of(chunk, krow) << 4) + (i & 1) * 8;
 #if defined(__HIP_DEVICE_COMPILE__)
         const s16x4 q = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
         const unsigned long long u = __builtin_bit_cast(unsigned long long, q);
@@ -152,7 +160,10 @@ struct Side {
     } else {
       u32x4 v = {};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = *(const uint32_t*)(tile + (kk * 8 + (lane >> 5) * 4 + j) * (R * E) + (r + (lane & 31)) * 4);
+      for (int j = 0; j < 4; ++j) {
+        const int krow = kk * 8 + (lane >> 5) * 4 + j, c = r + (lane & 31);
+        v[j] = *(const uint32_t*)(tile + krow * (R * E) + (slot_of(c >> 2, krow) << 4) + (c & 3) * 4);
+      }
       return v;
     }
   }
@@ -180,12 +191,16 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void token_tile_kernel(const TileA
   W sw;
   sx.init(a.x, a.ld_x, m0, a.M, k0);
   sw.init(a.w, a.ld_w, n0, a.N, k0);
-  const uint32_t l0 = lds_addr(smem);
-  int64_t k_left = a.K - (int64_t)k0 * X::KS;
-  auto fetch = [&](int stage) {
-    sx.fetch(l0 + stage * STAGE, k_left);
-    sw.fetch(l0 + stage * STAGE + BM * 128, k_left);
-    k_left -= X::KS;
+  const uint32_t l0 = __builtin_amdgcn_readfirstlane(lds_addr(smem) + (threadIdx.x & ~63u) * 16);      // this wave's lanes in each pass
+  const int64_t k_end = (int64_t)k1 * X::KS < a.K ? (int64_t)k1 * X::KS : a.K;
+  int64_t k_left = k_end - (int64_t)k0 * X::KS;
+  // one of the PX + PW pieces of the next step's tiles
+  constexpr int PX = X::PASSES, PW = W::PASSES;
+  auto open = [&]() { sx.open(); sw.open(); };
+  auto piece = [&](int i, int stage) {
+    const int left = k_left < 65536 ? (int)k_left : 65536;
+    if (i < PX) sx.piece(i, l0 + stage * STAGE, XS ? left : left * (int)sizeof(T));
+    else sw.piece(i - PX, l0 + stage * STAGE + BM * 128, WS ? left : left * (int)sizeof(T));
   };
   const int wave = threadIdx.x >> 6, wm = (wave % WM) * TM * 32, wn = (wave / WM) * TN * 32;
   f32x16 acc[TM][TN];
@@ -196,41 +211,58 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void token_tile_kernel(const TileA
 #pragma unroll
       for (int c = 0; c < 16; ++c) acc[i][j][c] = 0.f;
   u32x4 fx[2][TM], fw[2][TN];
-  auto read = [&](int set, int stage, int kk) {
+  auto read = [&](int set, int stage, int kk, int f) {      // fragment f of the TM + TN
     const char* s = smem + stage * STAGE;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) fx[set][i] = X::frag(s, wm + i * 32, kk);
-#pragma unroll
-    for (int j = 0; j < TN; ++j) fw[set][j] = W::frag(s + BM * 128, wn + j * 32, kk);
+    if (f < TM) fx[set][f] = X::frag(s, wm + f * 32, kk);
+    else fw[set][f - TM] = W::frag(s + BM * 128, wn + (f - TM) * 32, kk);
   };
-  auto mma = [&](int set) {
+  // a quarter of a step: the products of the fragments in `set`, between them one by one the reads of the next ones (and, in the
+  // last quarter, the fetches of the step after the next).  The compiler would sink the reads to their use; the order is kept.
+  auto quarter = [&](int set, int rstage, int rkk, bool last, int fstage) {
+    constexpr int NM = TM * TN, NF = TM + TN, RP = (NF + NM - 1) / NM, FP = (PX + PW + NM - 1) / NM;
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int p = 0; p < NM; ++p) {
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = Frag<T>::mma(fw[set][j], fx[set][i], acc[i][j]);
+      for (int f = p * RP; f < (p + 1) * RP; ++f)
+        if (f < NF) read(set ^ 1, rstage, rkk, f);
+      if (last) {
+#pragma unroll
+        for (int f = p * FP; f < (p + 1) * FP; ++f)
+          if (f < PX + PW) piece(f, fstage);
+      }
+      const int i = p % TM, j = p / TM;
+      acc[i][j] = Frag<T>::mma(fw[set][j], fx[set][i], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
 
   // The last quarter of a step is multiplied after the barrier that ends it: its fragments are in registers, and the reads of the
-  // next stage's first quarter, which only now may start, pass under those products.
+  // next stage's first quarter, which only now may start, pass under those products.  What is read or fetched past the last
+  // step is not used (fetches out of range leave zeros).
   if (k1 > k0) {
-    fetch(0);
-    barrier_all();
-    if (k1 - k0 > 1) fetch(1);
-    read(0, 0, 0);
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      open();
+#pragma unroll
+      for (int f = 0; f < PX + PW; ++f) piece(f, st);
+      k_left -= X::KS;
+      if (st == 0) barrier_all();
+    }
+#pragma unroll
+    for (int f = 0; f < TM + TN; ++f) read(0, 0, 0, f);
     int stage = 0;
+#pragma unroll 1
     for (int k = k0; k < k1; ++k) {
-      read(1, stage, 1);
-      mma(0);
-      read(0, stage, 2);
-      mma(1);
-      read(1, stage, 3);
-      mma(0);
+      quarter(0, stage, 1, false, 0);
+      quarter(1, stage, 2, false, 0);
+      quarter(0, stage, 3, false, 0);
       barrier_all();
-      if (k + 1 < k1) read(0, stage ^ 1, 0);
-      if (k + 2 < k1) fetch(stage);
-      mma(1);
+      open();
+      quarter(1, stage ^ 1, 0, true, stage);
+      k_left -= X::KS;
       stage ^= 1;
     }
+    barrier_all();
   }
 
   float* sh = (float*)smem + wave * (32 * PITCH);
@@ -315,8 +347,8 @@ __global__ __launch_bounds__(512, 1) void token_few_kernel(const FewArgs a) {
   __shared__ __attribute__((aligned(16))) float sh[8][MB * 16][20];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
-  const char* wrow = a.w + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ld_w;
   const char* xrow[MB];
+  const char* wrow = a.w + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ld_w;
 #pragma unroll
   for (int i = 0; i < MB; ++i) xrow[i] = a.x + (i * 16 + r < a.M ? i * 16 + r : a.M - 1) * a.ld_x;
   f32x4 acc[MB];
@@ -411,14 +443,15 @@ bool needs_pack(const Operand& o, int64_t rows, int64_t K, int E) {
   return ((uintptr_t)o.p & 15) || (o.ld * E) % 16 || (!o.padded && (inner * E) % 16) || outer * o.ld * E >= (1ll << 31) - 65536;
 }
 
-constexpr int64_t kFewRows = 64;
 constexpr int kTiles = 3;
 const int kTileM[kTiles] = {256, 128, 64}, kTileN[kTiles] = {256, 128, 64};
 
 Plan make_plan(const Product& p) {
   const int E = (int)dtype_bytes(p.dtype), V = 16 / E;
   Plan o = {};
-  if (!p.x.strided && !p.w.strided && p.M <= kFewRows) {
+  // token_few_kernel reads X again for every 16 columns, the tiles in whole tile rows: at 16 rows and 4096 x 4096 weights (bf16) 11.0 us
+  // against 14.7, at 32 rows 13.9 against 12.7; up to 64 rows where there is little to read at all (1024 x 1024: 7.0 against 8.3)
+  if (!p.x.strided && !p.w.strided && (p.M <= 16 || (p.M <= 64 && p.M * p.N * p.K <= 1 << 26))) {
     o.few = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
     return o;
   }
@@ -457,7 +490,10 @@ int run_tile(const TileArgs& a, hipStream_t st) {
 template <typename T, bool XS, bool WS>
 int run_tile_of(int tile, const TileArgs& a, hipStream_t st) {
   switch (tile) {
-    case 0: return run_tile<T, 4, 2, 2, 4, XS, WS>(a, st);
+#ifndef BIG
+#define BIG 4, 2, 2, 4
+#endif
+    case 0: return run_tile<T, BIG, XS, WS>(a, st);
     case 1: return run_tile<T, 2, 2, 2, 2, XS, WS>(a, st);
     default: return run_tile<T, 1, 1, 2, 2, XS, WS>(a, st);
   }

@@ -576,7 +576,7 @@ int sga_op_layer_norm_bwd(const sga_layer_norm* a, void* workspace, int64_t work
   const int st = norm_bwd_check(a);
   if (st != SGA_OK) return st;
   const int64_t need = norm_bwd_bytes(*a);
-  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))) return SGA_ERR_BAD_ARG;
+  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))) return SGA_ERR_NOMEM;
   hipStream_t s = (hipStream_t)stream;
   float* p = (float*)workspace;
   if (a->dtype == SGA_DTYPE_F32) return norm_bwd<float, float>(*a, p, s);

@@ -380,7 +380,8 @@ typedef struct sga_linear {
   void* g_x; void* g_w; void* g_bias;
   sga_dropout dropout;
 } sga_linear;
-/* bytes of DEVICE workspace (256-byte aligned) that the call with exactly these members needs; may be 0 */
+/* bytes of DEVICE workspace (256-byte aligned) that the call with exactly these members needs; may be 0.  A call whose workspace is
+ * missing, smaller or not aligned returns SGA_ERR_NOMEM and has done nothing */
 int sga_op_linear_workspace(const sga_linear* a, int backward, int64_t* bytes);
 int sga_op_linear_fwd(const sga_linear* a, void* workspace, int64_t workspace_bytes, void* stream);
 int sga_op_linear_bwd(const sga_linear* a, void* workspace, int64_t workspace_bytes, void* stream);

@@ -19,7 +19,7 @@ def linear(**kw):
     return a
 
 
-BAD, UNSUPPORTED = -1, -3
+BAD, UNSUPPORTED, NOMEM = -1, -3, -6
 
 
 @pytest.mark.parametrize("change,status", [
@@ -56,9 +56,9 @@ def test_linear_refuses_null_and_small_workspaces():
     assert lib.sga_op_linear_fwd(None, None, 0, None) == BAD
     a = linear(act=2, pre=P)
     assert lib.sga_op_linear_workspace(C.byref(a), 1, C.byref(n)) == 0 and n.value > 0
-    assert lib.sga_op_linear_bwd(C.byref(a), P, n.value - 1, None) == BAD
-    assert lib.sga_op_linear_bwd(C.byref(a), None, n.value, None) == BAD
-    assert lib.sga_op_linear_bwd(C.byref(a), P + 8, n.value, None) == BAD
+    assert lib.sga_op_linear_bwd(C.byref(a), P, n.value - 1, None) == NOMEM
+    assert lib.sga_op_linear_bwd(C.byref(a), None, n.value, None) == NOMEM
+    assert lib.sga_op_linear_bwd(C.byref(a), P + 8, n.value, None) == NOMEM
 
 
 def norm(**kw):
@@ -88,8 +88,8 @@ def test_layer_norm_refuses_by_direction():
     for change in ({"g_y": None}, {"mean": None}, {"rstd": None}, {"ld_g_y": 3}, {"g_add": P, "ld_g_add": 3}, {"g_x": P + 1}, {"g_w": P + 2}):
         assert lib.sga_op_layer_norm_bwd(C.byref(norm(**change)), P, 1 << 30, None) == BAD
     assert lib.sga_op_layer_norm_workspace(C.byref(norm()), 1, C.byref(n)) == 0 and n.value > 0
-    assert lib.sga_op_layer_norm_bwd(C.byref(norm()), P, n.value - 1, None) == BAD
-    assert lib.sga_op_layer_norm_bwd(C.byref(norm()), None, 0, None) == BAD
+    assert lib.sga_op_layer_norm_bwd(C.byref(norm()), P, n.value - 1, None) == NOMEM
+    assert lib.sga_op_layer_norm_bwd(C.byref(norm()), None, 0, None) == NOMEM
 
 
 def test_dropout_refuses():
@@ -129,8 +129,18 @@ def test_python_refuses_before_it_asks_for_a_gpu():
     for bad in ((-0.5, 1, 0), (1.5, 1, 0), (float("nan"), 1, 0), (0.5, 1), (0.5, torch.zeros(2))):
         with pytest.raises(ValueError):
             blocks._drop(bad, torch.device("cpu"))
-    d = blocks._drop((0.5, -1, 1 << 65), torch.device("cpu"))
-    assert d.seed == (1 << 64) - 1 and d.offset == 0
+    assert blocks._drop((0.5, -1, 1 << 65), torch.device("cpu")) == (0.5, (1 << 64) - 1, 0, 0)
+
+
+def test_packed_arguments_are_the_structures():
+    """blocks passes the structures of include/sga_hip.h as packed bytes: the same bytes as the ctypes structures hold."""
+    drop = (0.25, 3, 4, 5 << 12)
+    v = [7, 8, 9, 1, 2] + [P + 16 * i for i in range(15)]
+    a = _lib.SgaLinear(*v, _lib.SgaDropout(*drop))
+    assert blocks._LINEAR(*v, *drop) == bytes(a)
+    v = [7, 8, 1, 0, 0.5] + [P + 16 * i for i in range(14)]
+    assert blocks._NORM(*v) == bytes(_lib.SgaLayerNorm(*v))
+    assert blocks._DROPOUT(*drop) == bytes(_lib.SgaDropout(*drop))
 
 
 def test_row_layouts():
