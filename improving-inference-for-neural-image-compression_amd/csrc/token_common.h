@@ -172,64 +172,42 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float v
   *(t8*)p = a;
 }
 
-// columns n .. n + 7 of row m (those below e.cols); seed / offset: drop_key's
+// columns n .. n + 7 of row m, all of them there and aligned (e.vec); seed / offset: drop_key's
 template <typename T>
 __device__ __forceinline__ void epilogue8(const Epilogue& e, uint64_t seed, uint64_t offset, int64_t m, int64_t n, float v[8]) {
-  T* out = (T*)e.out + m * e.ld_out + n;
-  const T* res = e.residual ? (const T*)e.residual + m * e.ld_residual + n : nullptr;
-  T* pre = e.pre ? (T*)e.pre + m * e.cols + n : nullptr;
-  const T* bias = e.bias ? (const T*)e.bias + n : nullptr;
-  if (e.vec) {
-    if (n >= e.cols) return;
-    if (bias) {
-      float b[8];
-      load8(bias, b);
+  if (e.bias) {
+    float b[8];
+    load8((const T*)e.bias + n, b);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += b[j];
-    }
-    if (pre) store8(pre, v);
-    act_values<8>(v, e.act);
-    if (e.drop.on) {
-      const uint64_t g = (uint64_t)(m * e.cols + n) >> 2;      // cols and n are multiples of 8 here
-      uint32_t w[8];
-      drop_words(seed, offset, g, w);
-      drop_words(seed, offset, g + 1, w + 4);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = drop_apply(e.drop, w[j], v[j]);
-    }
-    if (res) {
-      float r[8];
-      load8(res, r);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += r[j];
-    }
-    store8(out, v);
-    return;
+    for (int j = 0; j < 8; ++j) v[j] += b[j];
   }
-  // pieces of any length and alignment, element by element; the 8 elements' words lie in three groups of four at most
-  const int live = e.cols - n < 8 ? (int)(e.cols - n) : 8;
-  uint32_t w[12];
-  const uint64_t i0 = (uint64_t)(m * e.cols + n);
-  const int shift = (int)(i0 & 3);
-  if (e.drop.on) {
-#pragma unroll
-    for (int g = 0; g < 3; ++g) drop_words(seed, offset, (i0 >> 2) + g, w + 4 * g);
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < live) {
-      if (bias) v[j] += to_f32(bias[j]);
-      if (pre) pre[j] = from_f32<T>(v[j]);
-    }
+  if (e.pre) store8((T*)e.pre + m * e.cols + n, v);
   act_values<8>(v, e.act);
+  if (e.drop.on) {
+    const uint64_t g = (uint64_t)(m * e.cols + n) >> 2;      // cols and n are multiples of 8 here
+    uint32_t w[8];
+    drop_words(seed, offset, g, w);
+    drop_words(seed, offset, g + 1, w + 4);
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < live) {
-      float u = v[j];
-      if (e.drop.on) u = drop_apply(e.drop, shift == 0 ? w[j] : shift == 1 ? w[j + 1] : shift == 2 ? w[j + 2] : w[j + 3], u);
-      if (res) u += to_f32(res[j]);
-      out[j] = from_f32<T>(u);
-    }
+    for (int j = 0; j < 8; ++j) v[j] = drop_apply(e.drop, w[j], v[j]);
+  }
+  if (e.residual) {
+    float r[8];
+    load8((const T*)e.residual + m * e.ld_residual + n, r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += r[j];
+  }
+  store8((T*)e.out + m * e.ld_out + n, v);
+}
+// one element, of any row length and alignment: lanes take neighbouring columns
+template <typename T>
+__device__ __forceinline__ void epilogue1(const Epilogue& e, uint64_t seed, uint64_t offset, int64_t m, int64_t n, float u) {
+  if (e.bias) u += to_f32(((const T*)e.bias)[n]);
+  if (e.pre) ((T*)e.pre)[m * e.cols + n] = from_f32<T>(u);
+  act_values<1>(&u, e.act);
+  if (e.drop.on) u = drop_one(e.drop, seed, offset, (uint64_t)(m * e.cols + n), u);
+  if (e.residual) u += to_f32(((const T*)e.residual)[m * e.ld_residual + n]);
+  ((T*)e.out)[m * e.ld_out + n] = from_f32<T>(u);
 }
 
 // ---- C[m, n] = epilogue(sum_k X(m, k) W(n, k)) (token_product.hip) -------------------------------------------------------

@@ -65,26 +65,40 @@ __device__ __forceinline__ void dma16(uint32_t lds, uint32_t voff, i32x4 srd) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(srd) : "memory");      // m0 is reserved: the compiler sets it before any use of its own
 #endif
 }
+// the same with 4 bytes per lane
+__device__ __forceinline__ void dma4(uint32_t lds, uint32_t voff, i32x4 srd) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(srd) : "memory");
+#endif
+}
 // everything this wave has in flight has landed, then all waves of the workgroup have got here
 __device__ __forceinline__ void barrier_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// the same, with the N latest fetches of this wave still on their way
+template <int N> __device__ __forceinline__ void barrier_but() {
+  static_assert(N >= 0 && N < 64, "the counter has 6 bits");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
 __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(lds_char*)p; }
 
 constexpr uint32_t kOutside = 0x80000000u;      // = num_records: a lane with this offset reads zeros
 
-// One operand's tile of R rows (m or n) per K step: how it is fetched and how its fragments are read
-template <typename T, int R, bool S, int NT>
+// One operand's tile of R rows (m or n) per K step: how it is fetched and how its fragments are read.  G: bytes that a lane fetches at
+// a time, 16, or 4 where rows are not made of aligned 16-byte pieces (then with four times the instructions)
+template <typename T, int R, bool S, int NT, int G>
 struct Side {
-  static constexpr int E = sizeof(T), KS = 128 / E, PASSES = R * 8 / NT, CPR = R * E / 16;      // KS: k per step; CPR: pieces per k row
-  static_assert(R * 8 % NT == 0 && NT % 128 == 0, "tile / threads");
-  // Where piece `chunk` of row `row` lies in LDS, and back.  64 banks of 4 bytes serve 256 bytes a cycle; the lanes of one cycle
-  // read  adjacent: 16 rows at one chunk | strided, 16 bit: 4 k rows x 2 neighbouring pairs of chunks | strided, 32 bit: 2 k rows, 4
-  // apart, x 8 chunks.  These keys put them on different banks (a row of 128 bytes gives the first bit by itself).
+  static constexpr int E = sizeof(T), KS = 128 / E, PASSES = R * 128 / (NT * G);      // KS: k per step
+  static constexpr int ROWB = S ? R * E : 128;                                        // bytes of an LDS row
+  static_assert(R * 128 % (NT * G) == 0 && NT % 128 == 0 && (G == 16 || G == 4) && G >= E, "tile / threads");
+
+  // Where 16-byte piece `chunk` of row `row` lies in LDS, and back.  64 banks of 4 bytes serve 256 bytes a cycle; the lanes of one
+  // cycle read  adjacent: 16 rows at one chunk | strided, 16 bit: 4 k rows x 2 neighbouring pairs of chunks | strided, 32 bit: 2 k
+  // rows, 4 apart, x 8 chunks.  These keys put them on different banks (a row of 128 bytes gives the first bit by itself).
   static __device__ __forceinline__ int key(int row) {
     if constexpr (!S) return (row >> 1) & 7;
     else if constexpr (E == 4) return ((row >> 2) & 1) << 3;
-    else return R * E == 128 ? ((row >> 1) & 1) << 2 : (row & 3) << 1;
+    else return ROWB == 128 ? ((row >> 1) & 1) << 2 : (row & 3) << 1;
   }
-  static constexpr bool FOLD = S && E == 2 && R * E > 128;      // the pair's lowest bit also goes into bit 3
+  static constexpr bool FOLD = S && E == 2 && ROWB > 128;      // the pair's lowest bit also goes into bit 3
   static __device__ __forceinline__ int slot_of(int chunk, int row) { return chunk ^ key(row) ^ (FOLD ? (chunk & 2) << 2 : 0); }
   static __device__ __forceinline__ int chunk_of(int slot, int row) {
     const int c = slot ^ key(row);
@@ -93,38 +107,40 @@ struct Side {
 
   const char* base;
   int64_t step;
-  uint32_t voff[PASSES];
-  int kpos[PASSES];         // strided: k row of the piece; adjacent: its offset in bytes (the same for all passes)
+  i32x4 srd;
+  uint32_t voff[PASSES];    // buffer offset of this lane's piece in each pass
+  int kpos;                 // and where along k the first one lies: adjacent, in bytes; strided, in rows
 
-  __device__ __forceinline__ void init(const char* p, int64_t ld, int64_t r0, int64_t rows, int kstep0) {
-    const int t = threadIdx.x;
+  static constexpr int STEP = NT * G / ROWB;      // LDS rows from pass to pass
+  static_assert(NT * G % ROWB == 0, "a pass takes whole rows");
+  // the same for pass i: the keys of rows STEP apart are the same, or differ in one bit
+  __device__ __forceinline__ int kpos_of(int i) const {
+    if constexpr (S) return kpos + i * STEP;
+    else return kpos ^ ((key(STEP) * i & 7) << 4);
+  }
+  __device__ __forceinline__ void init(const char* p, int64_t ld_, int64_t r0, int64_t rows, int kstep0) {
+    const uint32_t ld = (uint32_t)ld_;
+    int inner;                // strided: bytes of a k row from r0 on;  adjacent: the last row of the tile that exists
     if constexpr (!S) {
-      base = p + r0 * ld + (int64_t)kstep0 * 128;
+      base = p + r0 * ld_ + (int64_t)kstep0 * 128;
       step = 128;
-      const int chunk = chunk_of(t & 7, t >> 3);      // rows of one lane are NT / 8 apart: one key
-      const int64_t last = rows - 1 - r0;
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i) {
-        int64_t row = (i * NT + t) >> 3;
-        row = row < last ? row : last;
-        voff[i] = (uint32_t)(row * ld + chunk * 16);
-        kpos[i] = chunk * 16;
-      }
+      inner = rows - 1 - r0 < R ? (int)(rows - 1 - r0) : R;
     } else {
-      base = p + r0 * E + (int64_t)kstep0 * KS * ld;
-      step = (int64_t)KS * ld;
+      base = p + r0 * E + (int64_t)kstep0 * KS * ld_;
+      step = (int64_t)KS * ld_;
+      inner = (rows - r0) * E < R * E ? (int)(rows - r0) * E : R * E;
+    }
+    const int at = threadIdx.x * G, row0 = at / ROWB, col = at % ROWB;
+    kpos = S ? row0 : chunk_of(col >> 4, row0) * 16 + (col & 15);
 #pragma unroll
-      for (int i = 0; i < PASSES; ++i) {
-        const int idx = i * NT + t, krow = idx / CPR, slot = idx % CPR;
-        const int chunk = chunk_of(slot, krow);
-        voff[i] = (r0 * E + chunk * 16 < rows * E) ? (uint32_t)(krow * ld + chunk * 16) : kOutside;
-        kpos[i] = krow;
-      }
+    for (int i = 0; i < PASSES; ++i) {
+      const int row = row0 + i * STEP, b = chunk_of(col >> 4, row) * 16 + (col & 15);
+      if constexpr (!S) voff[i] = (uint32_t)(row < inner ? row : inner) * ld + b;
+      else voff[i] = b < inner ? row * ld + b : kOutside;
     }
   }
   // the next step's tile: open, then one piece after the other into LDS at `lds`; left: what of K there is from the step's start on, in
   // bytes (adjacent) or rows (strided), 0 or less: nothing
-  i32x4 srd;
   __device__ __forceinline__ void open() {
     const uint64_t b = (uint64_t)base;
     srd[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
@@ -134,13 +150,15 @@ struct Side {
     base += step;
   }
   __device__ __forceinline__ void piece(int i, uint32_t lds, int left) {
-    dma16(lds + i * NT * 16, kpos[i] < left ? voff[i] : kOutside, srd);
+    const uint32_t v = kpos_of(i) < left ? voff[i] : kOutside;
+    if constexpr (G == 16) dma16(lds + i * NT * 16, v, srd);
+    else dma4(lds + i * NT * 4, v, srd);
   }
   // fragment of the 32 rows from r on, k group kk (of 4): per lane 16 bytes = row (lane & 31), k = 16-byte piece 2 kk + (lane >> 5)
   static __device__ __forceinline__ u32x4 frag(const char* tile, int r, int kk) {
     const int lane = threadIdx.x & 63;
     if constexpr (!S) {
-      return *(const u32x4*)(tile + (r + (lane & 31)) * 128 + (slot_of(2 * kk + (lane >> 5), lane & 31) << 4));
+      return *(const u32x4*)(tile + (r + (lane & 31)) * ROWB + (slot_of(2 * kk + (lane >> 5), lane & 31) << 4));
     } else if constexpr (E == 2) {
       const int i = lane & 15, g = lane >> 4;
       u32x4 v = {};
@@ -148,8 +166,8 @@ struct Side {
       for (int h = 0; h < 2; ++h) {
         const int krow = kk * 16 + (g >> 1) * 8 + h * 4 + (i >> 2);
         const int chunk = (r >> 3) + (g & 1) * 2 + ((i & 3) >> 1);
-        const char* p = tile + krow * (R * E) + (slot_of(chunk, krow) << 4) + (i & 1) * 8;
 #if defined(__HIP_DEVICE_COMPILE__)
+        const char* p = tile + krow * ROWB + (slot_of(chunk, krow) << 4) + (i & 1) * 8;
         const s16x4 q = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
         const unsigned long long u = __builtin_bit_cast(unsigned long long, q);
         v[2 * h] = (unsigned)u;
@@ -162,19 +180,19 @@ struct Side {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int krow = kk * 8 + (lane >> 5) * 4 + j, c = r + (lane & 31);
-        v[j] = *(const uint32_t*)(tile + krow * (R * E) + (slot_of(c >> 2, krow) << 4) + (c & 3) * 4);
+        v[j] = *(const uint32_t*)(tile + krow * ROWB + (slot_of(c >> 2, krow) << 4) + (c & 3) * 4);
       }
       return v;
     }
   }
 };
 
-template <typename T, int TM, int TN, int WM, int WN, bool XS, bool WS>
+template <typename T, int TM, int TN, int WM, int WN, int NS, int G, bool XS, bool WS>
 __global__ __launch_bounds__(WM * WN * 64, 1) void token_tile_kernel(const TileArgs a) {
   constexpr int NT = WM * WN * 64, BM = WM * TM * 32, BN = WN * TN * 32, STAGE = (BM + BN) * 128;
   constexpr int PITCH = TN * 32 + 4;
-  typedef Side<T, BM, XS, NT> X;
-  typedef Side<T, BN, WS, NT> W;
+  typedef Side<T, BM, XS, NT, G> X;
+  typedef Side<T, BN, WS, NT, G> W;
   extern __shared__ __attribute__((aligned(16))) char smem[];
 
   // Blocks go to the 8 XCDs in turn; each XCD gets a contiguous run of tiles, walked in bands of 8 tile rows: the ~32 tiles that
@@ -191,7 +209,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void token_tile_kernel(const TileA
   W sw;
   sx.init(a.x, a.ld_x, m0, a.M, k0);
   sw.init(a.w, a.ld_w, n0, a.N, k0);
-  const uint32_t l0 = __builtin_amdgcn_readfirstlane(lds_addr(smem) + (threadIdx.x & ~63u) * 16);      // this wave's lanes in each pass
+  const uint32_t l0 = __builtin_amdgcn_readfirstlane(lds_addr(smem) + (threadIdx.x & ~63u) * G);      // this wave's lanes in each pass
   const int64_t k_end = (int64_t)k1 * X::KS < a.K ? (int64_t)k1 * X::KS : a.K;
   int64_t k_left = k_end - (int64_t)k0 * X::KS;
   // one of the PX + PW pieces of the next step's tiles
@@ -216,51 +234,59 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void token_tile_kernel(const TileA
     if (f < TM) fx[set][f] = X::frag(s, wm + f * 32, kk);
     else fw[set][f - TM] = W::frag(s + BM * 128, wn + (f - TM) * 32, kk);
   };
-  // a quarter of a step: the products of the fragments in `set`, between them one by one the reads of the next ones (and, in the
-  // last quarter, the fetches of the step after the next).  The compiler would sink the reads to their use; the order is kept.
-  auto quarter = [&](int set, int rstage, int rkk, bool last, int fstage) {
-    constexpr int NM = TM * TN, NF = TM + TN, RP = (NF + NM - 1) / NM, FP = (PX + PW + NM - 1) / NM;
+  // a quarter of a step: the products of the fragments in `set`, between them one by one the reads of the next ones and the fetches
+  // f0 .. f1 into stage fstage.  The compiler would sink the reads to their use; the order is kept.
+  auto quarter = [&](int set, int rstage, int rkk, int f0, int f1, int fstage) {
+    constexpr int NM = TM * TN, NF = TM + TN, RP = (NF + NM - 1) / NM;
+    const int FP = (f1 - f0 + NM - 1) / NM;
 #pragma unroll
     for (int p = 0; p < NM; ++p) {
 #pragma unroll
       for (int f = p * RP; f < (p + 1) * RP; ++f)
         if (f < NF) read(set ^ 1, rstage, rkk, f);
-      if (last) {
 #pragma unroll
-        for (int f = p * FP; f < (p + 1) * FP; ++f)
-          if (f < PX + PW) piece(f, fstage);
-      }
+      for (int f = f0 + p * FP; f < f0 + (p + 1) * FP; ++f)
+        if (f < f1) piece(f, fstage);
       const int i = p % TM, j = p / TM;
       acc[i][j] = Frag<T>::mma(fw[set][j], fx[set][i], acc[i][j]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  // The last quarter of a step is multiplied after the barrier that ends it: its fragments are in registers, and the reads of the
-  // next stage's first quarter, which only now may start, pass under those products.  What is read or fetched past the last
-  // step is not used (fetches out of range leave zeros).
+  // NS stages in a ring.  The last quarter of a step is multiplied after the barrier that ends it: its fragments are in registers, the
+  // reads of the next stage's first quarter, which only now may start, pass under those products, and so do the fetches of the
+  // step NS further on, into the stage that has just been read.  With two stages they are made at once, for they have three
+  // quarters to arrive; with more they are spread over the next four.  The barrier waits for the next stage's fetches alone;
+  // those of the NS - 2 stages after it stay on their way.  What is read or fetched past the last step is not used (fetches out
+  // of range leave zeros).
+  constexpr int P = PX + PW, Q1 = NS == 2 ? P : (P + 3) / 4, Q2 = NS == 2 ? P : (P + 1) / 2, Q3 = NS == 2 ? P : (3 * P + 3) / 4;
   if (k1 > k0) {
-#pragma unroll
-    for (int st = 0; st < 2; ++st) {
+#pragma unroll 1
+    for (int st = 0; st < NS - 1; ++st) {
       open();
 #pragma unroll
-      for (int f = 0; f < PX + PW; ++f) piece(f, st);
+      for (int f = 0; f < P; ++f) piece(f, st);
       k_left -= X::KS;
-      if (st == 0) barrier_all();
     }
+    open();
+#pragma unroll
+    for (int f = 0; f < Q1; ++f) piece(f, NS - 1);
+    barrier_but<(NS - 2) * P + Q1>();
 #pragma unroll
     for (int f = 0; f < TM + TN; ++f) read(0, 0, 0, f);
-    int stage = 0;
+    int stage = 0, prev = NS - 1;
 #pragma unroll 1
     for (int k = k0; k < k1; ++k) {
-      quarter(0, stage, 1, false, 0);
-      quarter(1, stage, 2, false, 0);
-      quarter(0, stage, 3, false, 0);
-      barrier_all();
-      open();
-      quarter(1, stage ^ 1, 0, true, stage);
+      const int next = stage + 1 == NS ? 0 : stage + 1;
+      quarter(0, stage, 1, Q1, Q2, prev);
+      quarter(1, stage, 2, Q2, Q3, prev);
+      quarter(0, stage, 3, Q3, P, prev);
+      barrier_but<(NS - 2) * P>();
       k_left -= X::KS;
-      stage ^= 1;
+      open();
+      quarter(1, next, 0, 0, Q1, stage);
+      prev = stage;
+      stage = next;
     }
     barrier_all();
   }
@@ -279,14 +305,23 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void token_tile_kernel(const TileA
         *(f32x4*)(sh + (lane & 31) * PITCH + j * 32 + c * 8 + (lane >> 5) * 4) =
             f32x4{acc[i][j][c * 4], acc[i][j][c * 4 + 1], acc[i][j][c * 4 + 2], acc[i][j][c * 4 + 3]};
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the rows below are other lanes' writes of this wave
+    if (a.e.vec || a.nsplit > 1) {
 #pragma unroll 1
-    for (int r = lane / LPR; r < 32; r += RPP) {
-      float v[8];
-      load8(sh + r * PITCH + (lane % LPR) * 8, v);
-      const int64_t m = m0 + wm + i * 32 + r, n = n0 + wn + (lane % LPR) * 8;
-      if (m >= a.M || n >= a.N) continue;
-      if (a.nsplit > 1) store8(a.part + ((int64_t)z * a.M + m) * a.ld_part + n, v);
-      else epilogue8<T>(a.e, seed, offset, m, n, v);
+      for (int r = lane / LPR; r < 32; r += RPP) {
+        float v[8];
+        load8(sh + r * PITCH + (lane % LPR) * 8, v);
+        const int64_t m = m0 + wm + i * 32 + r, n = n0 + wn + (lane % LPR) * 8;
+        if (m >= a.M || n >= a.N) continue;
+        if (a.nsplit > 1) store8(a.part + ((int64_t)z * a.M + m) * a.ld_part + n, v);
+        else epilogue8<T>(a.e, seed, offset, m, n, v);
+      }
+    } else {
+#pragma unroll 4
+      for (int r = 0; r < 16 * TN; ++r) {
+        const int at = r * 64 + lane, row = at / (TN * 32), col = at % (TN * 32);
+        const int64_t m = m0 + wm + i * 32 + row, n = n0 + wn + col;
+        if (m < a.M && n < a.N) epilogue1<T>(a.e, seed, offset, m, n, sh[row * PITCH + col]);
+      }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
@@ -376,37 +411,55 @@ __global__ __launch_bounds__(512, 1) void token_few_kernel(const FewArgs a) {
 #pragma unroll
   for (int i = 0; i < MB; ++i) *(f32x4*)&sh[wave][i * 16 + r][q * 4] = acc[i];
   __syncthreads();
-  const int m = threadIdx.x >> 1, c = (threadIdx.x & 1) * 8;
-  if (m >= a.M || n0 + c >= a.N) return;
-  float v[8], u[8];
-  load8(&sh[0][m][c], v);
-#pragma unroll
-  for (int s = 1; s < 8; ++s) {
-    load8(&sh[s][m][c], u);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] += u[j];
-  }
   uint64_t seed = 0, offset = 0;
   if (a.e.drop.on) drop_key(a.e.drop, seed, offset);
-  epilogue8<T>(a.e, seed, offset, m, n0 + c, v);
+  if (a.e.vec) {
+    const int m = threadIdx.x >> 1, c = (threadIdx.x & 1) * 8;
+    if (m >= a.M || n0 + c >= a.N) return;
+    float v[8], u[8];
+    load8(&sh[0][m][c], v);
+#pragma unroll
+    for (int s = 1; s < 8; ++s) {
+      load8(&sh[s][m][c], u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += u[j];
+    }
+    epilogue8<T>(a.e, seed, offset, m, n0 + c, v);
+  } else {
+    for (int i = threadIdx.x; i < MB * 256; i += 512) {
+      const int m = i >> 4, c = i & 15;
+      if (m >= a.M || n0 + c >= a.N) continue;
+      float v = sh[0][m][c];
+#pragma unroll
+      for (int s = 1; s < 8; ++s) v += sh[s][m][c];
+      epilogue1<T>(a.e, seed, offset, m, n0 + c, v);
+    }
+  }
 }
 
-// out = epilogue(sum of the slabs, in their order)
-template <typename T>
+// out = epilogue(sum of the slabs, in their order): 8 columns per lane, or one where the rows' pieces are not whole
+template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void token_join_kernel(const float* __restrict__ part, int nsplit, int64_t M, int64_t ld_part, const Epilogue e) {
-  const int64_t per = ld_part / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= M * per) return;
-  const int64_t m = i / per, n = (i - m * per) * 8;
   uint64_t seed = 0, offset = 0;
   if (e.drop.on) drop_key(e.drop, seed, offset);
-  float v[8], u[8];
-  load8(part + m * ld_part + n, v);
-  for (int s = 1; s < nsplit; ++s) {
-    load8(part + ((int64_t)s * M + m) * ld_part + n, u);
+  const int64_t per = VEC ? ld_part / 8 : e.cols, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= M * per) return;
+  const int64_t m = i / per, n = (i - m * per) * (VEC ? 8 : 1);
+  const float* p = part + m * ld_part + n;
+  if constexpr (VEC) {
+    float v[8], u[8];
+    load8(p, v);
+    for (int s = 1; s < nsplit; ++s) {
+      load8(p + s * M * ld_part, u);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] += u[j];
+      for (int j = 0; j < 8; ++j) v[j] += u[j];
+    }
+    epilogue8<T>(e, seed, offset, m, n, v);
+  } else {
+    float v = *p;
+    for (int s = 1; s < nsplit; ++s) v += p[s * M * ld_part];
+    epilogue1<T>(e, seed, offset, m, n, v);
   }
-  epilogue8<T>(e, seed, offset, m, n, v);
 }
 
 // dst [rows][cols_pad] = src [rows][cols], zeros behind: an operand whose rows are not 16-byte pieces
@@ -432,19 +485,26 @@ struct Plan {
   int few;                   // 16-row blocks of token_few_kernel, 0: tiles
   int tile;                  // index into the tile table
   int nsplit;
+  int fetch;                 // bytes per lane
   bool pack_x, pack_w;
   int64_t ldp_x, ldp_w;      // elements, packed
   int64_t x_off, w_off, part_off, bytes, ld_part;
 };
 
-bool needs_pack(const Operand& o, int64_t rows, int64_t K, int E) {
+// bytes that a lane can fetch at a time: all along rows of aligned pieces of 16, or of 4; 0: the operand has to be copied first.  A
+// tile's rows have to lie within the 2 GiB that an offset of the buffer descriptor spans.
+int fetch_bytes(const Operand& o, int64_t rows, int64_t K, int E) {
   const int64_t inner = o.strided ? rows : K, outer = o.strided ? 128 / E : 256;
-  // 16-byte pieces all along, and a tile's rows within the 2 GiB that an offset of the buffer descriptor spans
-  return ((uintptr_t)o.p & 15) || (o.ld * E) % 16 || (!o.padded && (inner * E) % 16) || outer * o.ld * E >= (1ll << 31) - 65536;
+  if (outer * o.ld * E >= (1ll << 31) - 65536) return 0;
+  const uint64_t bits = (uint64_t)(uintptr_t)o.p | (uint64_t)(o.ld * E);
+  if (!(bits & 15) && (o.padded || (inner * E) % 16 == 0)) return 16;
+  return !(bits & 3) && (o.padded || (inner * E) % 4 == 0) ? 4 : 0;
 }
 
-constexpr int kTiles = 3;
-const int kTileM[kTiles] = {256, 128, 64}, kTileN[kTiles] = {256, 128, 64};
+// tile, workgroups that are resident at a time, and the times of a K step and of everything else in a tile's life, in ns
+struct Tile { int m, n, slots; double step16, step32, once; };
+constexpr int kTiles = 4;
+const Tile kTile[kTiles] = {{256, 256, 256, 1650, 14500, 11000}, {256, 128, 256, 1050, 7600, 8000}, {128, 128, 256, 620, 4000, 5000}, {64, 64, 512, 500, 1900, 3000}};
 
 Plan make_plan(const Product& p) {
   const int E = (int)dtype_bytes(p.dtype), V = 16 / E;
@@ -455,21 +515,21 @@ Plan make_plan(const Product& p) {
     o.few = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
     return o;
   }
-  o.pack_x = needs_pack(p.x, p.M, p.K, E);
-  o.pack_w = needs_pack(p.w, p.N, p.K, E);
+  const int gx = fetch_bytes(p.x, p.M, p.K, E), gw = fetch_bytes(p.w, p.N, p.K, E);
+  o.pack_x = gx == 0;
+  o.pack_w = gw == 0;
+  o.fetch = gx == 4 || gw == 4 ? 4 : 16;
   if (o.pack_x) { o.ldp_x = round_up(p.x.strided ? p.M : p.K, V); o.x_off = o.bytes; o.bytes += round_up((p.x.strided ? p.K : p.M) * o.ldp_x * E, 256); }
   if (o.pack_w) { o.ldp_w = round_up(p.w.strided ? p.N : p.K, V); o.w_off = o.bytes; o.bytes += round_up((p.w.strided ? p.K : p.N) * o.ldp_w * E, 256); }
   const int64_t nk = ceil_div(p.K, 128 / E);
   double best = 1e300;
   o.nsplit = 1;
   for (int t = 0; t < kTiles; ++t) {
-    const int64_t tiles = ceil_div(p.M, kTileM[t]) * ceil_div(p.N, kTileN[t]);
-    static const int slots[kTiles] = {256, 512, 1024};
-    static const double per_step[kTiles] = {1.0, 0.62, 0.34};      // time of a K step of one workgroup with its CU shared by the others, relative
-    for (int s = 1; s == 1 || (s <= 16 && s <= nk); s *= 2) {
-      const double rounds = (double)ceil_div(tiles * s, slots[t]);
-      double cost = rounds * ((double)ceil_div(nk, s) + 4.0) * per_step[t];
-      if (s > 1) cost += 4.0 + (double)p.M * p.N * s * 8.0 / 4e12 / 0.9e-6;
+    const int64_t tiles = ceil_div(p.M, kTile[t].m) * ceil_div(p.N, kTile[t].n);
+    for (int s = 1; s == 1 || (s <= 16 && s <= nk); ++s) {
+      const double rounds = (double)ceil_div(tiles * s, kTile[t].slots);
+      double cost = rounds * ((double)ceil_div(nk, s) * (E == 4 ? kTile[t].step32 : kTile[t].step16) + kTile[t].once);
+      if (s > 1) cost += 4000.0 + (double)p.M * p.N * (s * 8.0 + E) / 3500.0;      // the slabs' way out and back at 3.5 TB/s, a launch
       if (cost < best) { best = cost; o.tile = t; o.nsplit = s; }
     }
   }
@@ -477,26 +537,30 @@ Plan make_plan(const Product& p) {
   return o;
 }
 
-template <typename T, int TM, int TN, int WM, int WN, bool XS, bool WS>
+template <typename T, int TM, int TN, int WM, int WN, int NS, int G, bool XS, bool WS>
 int run_tile(const TileArgs& a, hipStream_t st) {
-  constexpr int BM = WM * TM * 32, BN = WN * TN * 32, MAIN = 2 * (BM + BN) * 128, EPI = WM * WN * 32 * (TN * 32 + 4) * 4;
+  constexpr int BM = WM * TM * 32, BN = WN * TN * 32, MAIN = NS * (BM + BN) * 128, EPI = WM * WN * 32 * (TN * 32 + 4) * 4;
   constexpr int LDS = MAIN > EPI ? MAIN : EPI;
-  const void* f = reinterpret_cast<const void*>(&token_tile_kernel<T, TM, TN, WM, WN, XS, WS>);
+  const void* f = reinterpret_cast<const void*>(&token_tile_kernel<T, TM, TN, WM, WN, NS, G, XS, WS>);
   if (LDS > 65536 && hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return SGA_ERR_HIP;
-  hipLaunchKernelGGL((token_tile_kernel<T, TM, TN, WM, WN, XS, WS>), dim3((unsigned)(a.ntm * a.ntn * a.nsplit)), dim3(WM * WN * 64), LDS, st, a);
+  hipLaunchKernelGGL((token_tile_kernel<T, TM, TN, WM, WN, NS, G, XS, WS>), dim3((unsigned)(a.ntm * a.ntn * a.nsplit)), dim3(WM * WN * 64), LDS, st, a);
   LAUNCHED();
   return SGA_OK;
 }
-template <typename T, bool XS, bool WS>
+template <typename T, int G, bool XS, bool WS>
 int run_tile_of(int tile, const TileArgs& a, hipStream_t st) {
   switch (tile) {
-#ifndef BIG
-#define BIG 4, 2, 2, 4
-#endif
-    case 0: return run_tile<T, BIG, XS, WS>(a, st);
-    case 1: return run_tile<T, 2, 2, 2, 2, XS, WS>(a, st);
-    default: return run_tile<T, 1, 1, 2, 2, XS, WS>(a, st);
+    case 0: return run_tile<T, 2, 4, 4, 2, 2, G, XS, WS>(a, st);
+    case 1: return run_tile<T, 2, 2, 4, 2, 3, G, XS, WS>(a, st);
+    case 2: return run_tile<T, 1, 2, 4, 2, 4, G, XS, WS>(a, st);
+    default: return run_tile<T, 1, 1, 2, 2, 4, G, XS, WS>(a, st);
   }
+}
+template <typename T, int G>
+int run_order(int tile, bool xs, bool ws, const TileArgs& a, hipStream_t st) {
+  if (!xs && !ws) return run_tile_of<T, G, false, false>(tile, a, st);
+  if (!xs) return run_tile_of<T, G, false, true>(tile, a, st);
+  return run_tile_of<T, G, true, true>(tile, a, st);
 }
 
 template <typename T, int MB>
@@ -535,18 +599,19 @@ int run(const Product& p, char* ws, hipStream_t st) {
   if (s != SGA_OK) return s;
   a.M = p.M; a.N = p.N; a.K = p.K;
   a.nk = (int)ceil_div(p.K, 128 / (int)sizeof(T));
-  a.ntm = (int)ceil_div(p.M, kTileM[o.tile]);
-  a.ntn = (int)ceil_div(p.N, kTileN[o.tile]);
+  a.ntm = (int)ceil_div(p.M, kTile[o.tile].m);
+  a.ntn = (int)ceil_div(p.N, kTile[o.tile].n);
   a.nsplit = o.nsplit;
   a.part = o.nsplit > 1 ? (float*)(ws + o.part_off) : nullptr;
   a.ld_part = o.ld_part;
   a.e = p.e;
   if ((int64_t)a.ntm * a.ntn * a.nsplit > 0x7fffffff) return SGA_ERR_UNSUPPORTED;
-  if (!p.x.strided && !p.w.strided) s = run_tile_of<T, false, false>(o.tile, a, st);
-  else if (!p.x.strided) s = run_tile_of<T, false, true>(o.tile, a, st);
-  else s = run_tile_of<T, true, true>(o.tile, a, st);
+  s = o.fetch == 16 ? run_order<T, 16>(o.tile, p.x.strided, p.w.strided, a, st) : run_order<T, 4>(o.tile, p.x.strided, p.w.strided, a, st);
   if (s != SGA_OK || o.nsplit == 1) return s;
-  hipLaunchKernelGGL((token_join_kernel<T>), dim3((unsigned)ceil_div(p.M * (o.ld_part / 8), 256)), dim3(256), 0, st, a.part, o.nsplit, p.M, o.ld_part, p.e);
+  if (p.e.vec)
+    hipLaunchKernelGGL((token_join_kernel<T, true>), dim3((unsigned)ceil_div(p.M * (o.ld_part / 8), 256)), dim3(256), 0, st, a.part, o.nsplit, p.M, o.ld_part, p.e);
+  else
+    hipLaunchKernelGGL((token_join_kernel<T, false>), dim3((unsigned)ceil_div(p.M * p.N, 256)), dim3(256), 0, st, a.part, o.nsplit, p.M, o.ld_part, p.e);
   LAUNCHED();
   return SGA_OK;
 }
