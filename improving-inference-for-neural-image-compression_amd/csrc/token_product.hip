@@ -37,24 +37,32 @@ struct TileArgs {
   Epilogue e;
 };
 
-template <typename T> struct Frag;
-template <> struct Frag<bf16> {
-  typedef bf16 v8 __attribute__((ext_vector_type(8)));
-  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+// The matrix instructions by type and size MF (32 x 32 or 16 x 16 results, 16 or 4 per lane): one takes 16 bytes per lane of either
+// operand, row lane % MF, bytes 16 (lane / MF) .. of a group of 1024 / MF bytes along k (32-bit types: four instructions, j)
+template <typename T, int MF> struct Mma;
+#define MMA(T, MF, RES, CALL)                                                     \
+  template <> struct Mma<T, MF> {                                                 \
+    typedef T v8 __attribute__((ext_vector_type(8)));                             \
+    typedef RES acc;                                                              \
+    static __device__ __forceinline__ acc mma1(u32x4 a, u32x4 b, int, acc c) {    \
+      return CALL(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0); \
+    }                                                                             \
+  }
+MMA(bf16, 32, f32x16, __builtin_amdgcn_mfma_f32_32x32x16_bf16);
+MMA(f16, 32, f32x16, __builtin_amdgcn_mfma_f32_32x32x16_f16);
+MMA(bf16, 16, f32x4, __builtin_amdgcn_mfma_f32_16x16x32_bf16);
+MMA(f16, 16, f32x4, __builtin_amdgcn_mfma_f32_16x16x32_f16);
+#undef MMA
+template <> struct Mma<float, 32> {
+  typedef f32x16 acc;
+  static __device__ __forceinline__ acc mma1(u32x4 a, u32x4 b, int j, acc c) {
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
   }
 };
-template <> struct Frag<f16> {
-  typedef f16 v8 __attribute__((ext_vector_type(8)));
-  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
-  }
-};
-template <> struct Frag<float> {
-  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
-    return c;
+template <> struct Mma<float, 16> {
+  typedef f32x4 acc;
+  static __device__ __forceinline__ acc mma1(u32x4 a, u32x4 b, int j, acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
   }
 };
 
@@ -84,18 +92,18 @@ constexpr uint32_t kOutside = 0x80000000u;      // = num_records: a lane with th
 
 // One operand's tile of R rows (m or n) per K step: how it is fetched and how its fragments are read.  G: bytes that a lane fetches at
 // a time, 16, or 4 where rows are not made of aligned 16-byte pieces (then with four times the instructions)
-template <typename T, int R, bool S, int NT, int G>
+template <typename T, int R, bool S, int NT, int G, int MF>
 struct Side {
   static constexpr int E = sizeof(T), KS = 128 / E, PASSES = R * 128 / (NT * G);      // KS: k per step
   static constexpr int ROWB = S ? R * E : 128;                                        // bytes of an LDS row
-  static_assert(R * 128 % (NT * G) == 0 && NT % 128 == 0 && (G == 16 || G == 4) && G >= E, "tile / threads");
+  static_assert(R * 128 % (NT * G) == 0 && NT % 128 == 0 && (S || R % MF == 0) && (G == 16 || G == 4) && G >= E, "tile / threads");
 
   // Where 16-byte piece `chunk` of row `row` lies in LDS, and back.  64 banks of 4 bytes serve 256 bytes a cycle; the lanes of one
-  // cycle read  adjacent: 16 rows at one chunk | strided, 16 bit: 4 k rows x 2 neighbouring pairs of chunks | strided, 32 bit: 2 k
-  // rows, 4 apart, x 8 chunks.  These keys put them on different banks (a row of 128 bytes gives the first bit by itself).
+  // cycle read  adjacent: 16 rows at one chunk | strided, 16 bit: 4 k rows x 2 neighbouring pairs of chunks | strided, 32 bit: 2 (4) k
+  // rows, 4 apart, x 8 (4) chunks.  These keys put them on different banks (a row of 128 bytes gives the first bit by itself).
   static __device__ __forceinline__ int key(int row) {
     if constexpr (!S) return (row >> 1) & 7;
-    else if constexpr (E == 4) return ((row >> 2) & 1) << 3;
+    else if constexpr (E == 4) return MF == 32 ? ((row >> 2) & 1) << 3 : ((row >> 2) & 3) << 2;
     else return ROWB == 128 ? ((row >> 1) & 1) << 2 : (row & 3) << 1;
   }
   static constexpr bool FOLD = S && E == 2 && ROWB > 128;      // the pair's lowest bit also goes into bit 3
@@ -154,45 +162,44 @@ struct Side {
     if constexpr (G == 16) dma16(lds + i * NT * 16, v, srd);
     else dma4(lds + i * NT * 4, v, srd);
   }
-  // fragment of the 32 rows from r on, k group kk (of 4): per lane 16 bytes = row (lane & 31), k = 16-byte piece 2 kk + (lane >> 5)
+  // fragment of the MF rows from r on, k group kk, for Mma<T, MF>
   static __device__ __forceinline__ u32x4 frag(const char* tile, int r, int kk) {
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, rl = lane % MF, kl = lane / MF;
+    u32x4 v = {};
     if constexpr (!S) {
-      return *(const u32x4*)(tile + (r + (lane & 31)) * ROWB + (slot_of(2 * kk + (lane >> 5), lane & 31) << 4));
+      v = *(const u32x4*)(tile + (r + rl) * ROWB + (slot_of(kk * (64 / MF) + kl, rl) << 4));
     } else if constexpr (E == 2) {
-      const int i = lane & 15, g = lane >> 4;
-      u32x4 v = {};
+#if defined(__HIP_DEVICE_COMPILE__)
+      // 16 lanes hand in 4 k rows x 16 elements and get 4 k of one element each
+      const int i = lane & 15, half = MF == 32 ? (lane >> 4) & 1 : 0;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int krow = kk * 16 + (g >> 1) * 8 + h * 4 + (i >> 2);
-        const int chunk = (r >> 3) + (g & 1) * 2 + ((i & 3) >> 1);
-#if defined(__HIP_DEVICE_COMPILE__)
+        const int krow = kk * (512 / MF) + kl * 8 + h * 4 + (i >> 2), chunk = (r >> 3) + half * 2 + ((i & 3) >> 1);
         const char* p = tile + krow * ROWB + (slot_of(chunk, krow) << 4) + (i & 1) * 8;
         const s16x4 q = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
         const unsigned long long u = __builtin_bit_cast(unsigned long long, q);
         v[2 * h] = (unsigned)u;
         v[2 * h + 1] = (unsigned)(u >> 32);
-#endif
       }
-      return v;
+#endif
     } else {
-      u32x4 v = {};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int krow = kk * 8 + (lane >> 5) * 4 + j, c = r + (lane & 31);
+        const int krow = kk * (256 / MF) + kl * 4 + j, c = r + rl;
         v[j] = *(const uint32_t*)(tile + krow * ROWB + (slot_of(c >> 2, krow) << 4) + (c & 3) * 4);
       }
-      return v;
     }
+    return v;
   }
 };
 
-template <typename T, int TM, int TN, int WM, int WN, int NS, int G, bool XS, bool WS>
-__global__ __launch_bounds__(WM * WN * 64, 1) void token_tile_kernel(const TileArgs a) {
-  constexpr int NT = WM * WN * 64, BM = WM * TM * 32, BN = WN * TN * 32, STAGE = (BM + BN) * 128;
-  constexpr int PITCH = TN * 32 + 4;
-  typedef Side<T, BM, XS, NT, G> X;
-  typedef Side<T, BN, WS, NT, G> W;
+template <typename T, int MF, int TM, int TN, int WM, int WN, int NS, int G, bool XS, bool WS>
+__global__ __launch_bounds__(WM * WN * 64, 2) void token_tile_kernel(const TileArgs a) {
+  constexpr int NT = WM * WN * 64, BM = WM * TM * MF, BN = WN * TN * MF, STAGE = (BM + BN) * 128;
+  constexpr int PITCH = TN * MF + 4;
+  typedef Side<T, BM, XS, NT, G, MF> X;
+  typedef Side<T, BN, WS, NT, G, MF> W;
+  typedef Mma<T, MF> I;
   extern __shared__ __attribute__((aligned(16))) char smem[];
 
   // Blocks go to the 8 XCDs in turn; each XCD gets a contiguous run of tiles, walked in bands of 8 tile rows: the ~32 tiles that
@@ -220,46 +227,43 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void token_tile_kernel(const TileA
     if (i < PX) sx.piece(i, l0 + stage * STAGE, XS ? left : left * (int)sizeof(T));
     else sw.piece(i - PX, l0 + stage * STAGE + BM * 128, WS ? left : left * (int)sizeof(T));
   };
-  const int wave = threadIdx.x >> 6, wm = (wave % WM) * TM * 32, wn = (wave / WM) * TN * 32;
-  f32x16 acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int c = 0; c < 16; ++c) acc[i][j][c] = 0.f;
+  const int wave = threadIdx.x >> 6, wm = (wave % WM) * TM * MF, wn = (wave / WM) * TN * MF;
+  // NJ instructions per pair of fragments, each over all pairs before the next: an instruction that adds to what the last one left
+  // waits for it.  A single pair has two sums in turn.
+  constexpr int NM = TM * TN, NJ = sizeof(T) == 4 ? 4 : 1, ND = NM == 1 && NJ > 1 ? 2 : 1;
+  typename I::acc acc[TM][TN][ND] = {};
   u32x4 fx[2][TM], fw[2][TN];
   auto read = [&](int set, int stage, int kk, int f) {      // fragment f of the TM + TN
     const char* s = smem + stage * STAGE;
-    if (f < TM) fx[set][f] = X::frag(s, wm + f * 32, kk);
-    else fw[set][f - TM] = W::frag(s + BM * 128, wn + (f - TM) * 32, kk);
+    if (f < TM) fx[set][f] = X::frag(s, wm + f * MF, kk);
+    else fw[set][f - TM] = W::frag(s + BM * 128, wn + (f - TM) * MF, kk);
   };
-  // a quarter of a step: the products of the fragments in `set`, between them one by one the reads of the next ones and the fetches
+  // one k group of a step: the products of the fragments in `set`, between them one by one the reads of the next ones and the fetches
   // f0 .. f1 into stage fstage.  The compiler would sink the reads to their use; the order is kept.
-  auto quarter = [&](int set, int rstage, int rkk, int f0, int f1, int fstage) {
-    constexpr int NM = TM * TN, NF = TM + TN, RP = (NF + NM - 1) / NM;
-    const int FP = (f1 - f0 + NM - 1) / NM;
+  auto group = [&](int set, int rstage, int rkk, int f0, int f1, int fstage) {
+    constexpr int NF = TM + TN, RP = (NF + NM * NJ - 1) / (NM * NJ);
 #pragma unroll
-    for (int p = 0; p < NM; ++p) {
+    for (int q = 0; q < NM * NJ; ++q) {
 #pragma unroll
-      for (int f = p * RP; f < (p + 1) * RP; ++f)
+      for (int f = q * RP; f < (q + 1) * RP; ++f)
         if (f < NF) read(set ^ 1, rstage, rkk, f);
 #pragma unroll
-      for (int f = f0 + p * FP; f < f0 + (p + 1) * FP; ++f)
-        if (f < f1) piece(f, fstage);
-      const int i = p % TM, j = p / TM;
-      acc[i][j] = Frag<T>::mma(fw[set][j], fx[set][i], acc[i][j]);
+      for (int f = f0; f < f1; ++f)
+        if ((f - f0) * NM * NJ / (f1 - f0) == q) piece(f, fstage);
+      const int i = q % NM % TM, j = q % NM / TM;
+      acc[i][j][q / NM % ND] = I::mma1(fw[set][j], fx[set][i], q / NM, acc[i][j][q / NM % ND]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  // NS stages in a ring.  The last quarter of a step is multiplied after the barrier that ends it: its fragments are in registers, the
-  // reads of the next stage's first quarter, which only now may start, pass under those products, and so do the fetches of the
-  // step NS further on, into the stage that has just been read.  With two stages they are made at once, for they have three
-  // quarters to arrive; with more they are spread over the next four.  The barrier waits for the next stage's fetches alone;
-  // those of the NS - 2 stages after it stay on their way.  What is read or fetched past the last step is not used (fetches out
-  // of range leave zeros).
-  constexpr int P = PX + PW, Q1 = NS == 2 ? P : (P + 3) / 4, Q2 = NS == 2 ? P : (P + 1) / 2, Q3 = NS == 2 ? P : (3 * P + 3) / 4;
+  // NS stages in a ring, NG k groups a step.  The last group of a step is multiplied after the barrier that ends it: its fragments are
+  // in registers, the reads of the next stage's first group, which only now may start, pass under those products, and so do the
+  // fetches of the step NS further on, into the stage that has just been read.  With two stages they are made at once, for
+  // they have less than a step to arrive; with more they are spread over the next NG groups.  The barrier waits for the next
+  // stage's fetches alone; those of the NS - 2 stages after it stay on their way.  What is read or fetched past the last step is
+  // not used (fetches out of range leave zeros).
+  constexpr int P = PX + PW, NG = MF / 8, Q = NS == 2 ? P : (P + NG - 1) / NG;      // fetches in a group
+  constexpr auto upto = [](int g) { return g * Q < P ? g * Q : P; };
   if (k1 > k0) {
 #pragma unroll 1
     for (int st = 0; st < NS - 1; ++st) {
@@ -270,56 +274,58 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void token_tile_kernel(const TileA
     }
     open();
 #pragma unroll
-    for (int f = 0; f < Q1; ++f) piece(f, NS - 1);
-    barrier_but<(NS - 2) * P + Q1>();
+    for (int f = 0; f < Q; ++f) piece(f, NS - 1);
+    barrier_but<(NS - 2) * P + Q>();
 #pragma unroll
     for (int f = 0; f < TM + TN; ++f) read(0, 0, 0, f);
     int stage = 0, prev = NS - 1;
 #pragma unroll 1
     for (int k = k0; k < k1; ++k) {
       const int next = stage + 1 == NS ? 0 : stage + 1;
-      quarter(0, stage, 1, Q1, Q2, prev);
-      quarter(1, stage, 2, Q2, Q3, prev);
-      quarter(0, stage, 3, Q3, P, prev);
+#pragma unroll
+      for (int g = 0; g < NG - 1; ++g) group(g & 1, stage, g + 1, upto(g + 1), upto(g + 2), prev);
       barrier_but<(NS - 2) * P>();
       k_left -= X::KS;
       open();
-      quarter(1, next, 0, 0, Q1, stage);
+      group((NG - 1) & 1, next, 0, 0, upto(1), stage);
       prev = stage;
       stage = next;
     }
     barrier_all();
   }
 
-  float* sh = (float*)smem + wave * (32 * PITCH);
+  if constexpr (ND == 2) acc[0][0][0] += acc[0][0][ND - 1];
+
+  // this wave's results, MF rows at a time, through LDS to lanes of neighbouring columns
+  float* sh = (float*)smem + wave * (MF * PITCH);
   const int lane = threadIdx.x & 63;
   uint64_t seed = 0, offset = 0;
   if (a.e.drop.on) drop_key(a.e.drop, seed, offset);
-  constexpr int LPR = TN * 4, RPP = 64 / LPR;      // lanes per row of 8-column pieces, rows per pass
+  constexpr int COLS = TN * MF, LPR = COLS / 8;      // lanes per row of 8-column pieces
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        *(f32x4*)(sh + (lane & 31) * PITCH + j * 32 + c * 8 + (lane >> 5) * 4) =
-            f32x4{acc[i][j][c * 4], acc[i][j][c * 4 + 1], acc[i][j][c * 4 + 2], acc[i][j][c * 4 + 3]};
+      for (int c = 0; c < MF * MF / 256; ++c)
+        *(f32x4*)(sh + (lane % MF) * PITCH + j * MF + c * 8 + (lane / MF) * 4) =
+            f32x4{acc[i][j][0][c * 4], acc[i][j][0][c * 4 + 1], acc[i][j][0][c * 4 + 2], acc[i][j][0][c * 4 + 3]};
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the rows below are other lanes' writes of this wave
     if (a.e.vec || a.nsplit > 1) {
 #pragma unroll 1
-      for (int r = lane / LPR; r < 32; r += RPP) {
+      for (int r = lane / LPR; r < MF; r += 64 / LPR) {
         float v[8];
         load8(sh + r * PITCH + (lane % LPR) * 8, v);
-        const int64_t m = m0 + wm + i * 32 + r, n = n0 + wn + (lane % LPR) * 8;
+        const int64_t m = m0 + wm + i * MF + r, n = n0 + wn + (lane % LPR) * 8;
         if (m >= a.M || n >= a.N) continue;
         if (a.nsplit > 1) store8(a.part + ((int64_t)z * a.M + m) * a.ld_part + n, v);
         else epilogue8<T>(a.e, seed, offset, m, n, v);
       }
     } else {
 #pragma unroll 4
-      for (int r = 0; r < 16 * TN; ++r) {
-        const int at = r * 64 + lane, row = at / (TN * 32), col = at % (TN * 32);
-        const int64_t m = m0 + wm + i * 32 + row, n = n0 + wn + col;
+      for (int r = 0; r < MF * COLS / 64; ++r) {
+        const int at = r * 64 + lane, row = at / COLS, col = at % COLS;
+        const int64_t m = m0 + wm + i * MF + row, n = n0 + wn + col;
         if (m < a.M && n < a.N) epilogue1<T>(a.e, seed, offset, m, n, sh[row * PITCH + col]);
       }
     }
@@ -331,27 +337,6 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void token_tile_kernel(const TileA
 // A workgroup of 8 waves owns 16 columns n.  The waves share out K in pieces of 128 bytes per row of w, so that a wave reads whole
 // lines; MFMA rows = the 16 columns, MFMA columns = 16 rows of X (MB of them).  Any order of k inside a piece serves, as both
 // operands take the same: lane (r, q) takes bytes q * 16 .. of each 64.  The waves' sums meet in LDS.
-template <typename T> struct Frag16;
-template <> struct Frag16<bf16> {
-  typedef bf16 v8 __attribute__((ext_vector_type(8)));
-  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
-  }
-};
-template <> struct Frag16<f16> {
-  typedef f16 v8 __attribute__((ext_vector_type(8)));
-  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
-  }
-};
-template <> struct Frag16<float> {
-  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
-    return c;
-  }
-};
-
 struct FewArgs {
   const char* x; const char* w;
   int64_t ld_x, ld_w;            // bytes
@@ -406,7 +391,9 @@ __global__ __launch_bounds__(512, 1) void token_few_kernel(const FewArgs a) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < MB; ++i) acc[i] = Frag16<T>::mma(fw[u][h], fx[u][h][i], acc[i]);
+        for (int j = 0; j < (sizeof(T) == 4 ? 4 : 1); ++j)
+#pragma unroll
+          for (int i = 0; i < MB; ++i) acc[i] = Mma<T, 16>::mma1(fw[u][h], fx[u][h][i], j, acc[i]);
   }
 #pragma unroll
   for (int i = 0; i < MB; ++i) *(f32x4*)&sh[wave][i * 16 + r][q * 4] = acc[i];
@@ -503,8 +490,8 @@ int fetch_bytes(const Operand& o, int64_t rows, int64_t K, int E) {
 
 // tile, workgroups that are resident at a time, and the times of a K step and of everything else in a tile's life, in ns
 struct Tile { int m, n, slots; double step16, step32, once; };
-constexpr int kTiles = 4;
-const Tile kTile[kTiles] = {{256, 256, 256, 1650, 14500, 11000}, {256, 128, 256, 1050, 7600, 8000}, {128, 128, 256, 620, 4000, 5000}, {64, 64, 512, 500, 1900, 3000}};
+constexpr int kTiles = 5;
+const Tile kTile[kTiles] = {{256, 256, 256, 1650, 14500, 11000}, {256, 128, 256, 1050, 7600, 8000}, {128, 128, 256, 620, 4000, 5000}, {96, 64, 512, 600, 2500, 3000}, {64, 64, 512, 500, 1900, 3000}};
 
 Plan make_plan(const Product& p) {
   const int E = (int)dtype_bytes(p.dtype), V = 16 / E;
@@ -525,6 +512,7 @@ Plan make_plan(const Product& p) {
   double best = 1e300;
   o.nsplit = 1;
   for (int t = 0; t < kTiles; ++t) {
+    if (kTile[t].m == 96 && p.x.strided) continue;      // the keys of a k row need a power of two
     const int64_t tiles = ceil_div(p.M, kTile[t].m) * ceil_div(p.N, kTile[t].n);
     for (int s = 1; s == 1 || (s <= 16 && s <= nk); ++s) {
       const double rounds = (double)ceil_div(tiles * s, kTile[t].slots);
@@ -537,23 +525,26 @@ Plan make_plan(const Product& p) {
   return o;
 }
 
-template <typename T, int TM, int TN, int WM, int WN, int NS, int G, bool XS, bool WS>
+template <typename T, int MF, int TM, int TN, int WM, int WN, int NS, int G, bool XS, bool WS>
 int run_tile(const TileArgs& a, hipStream_t st) {
-  constexpr int BM = WM * TM * 32, BN = WN * TN * 32, MAIN = NS * (BM + BN) * 128, EPI = WM * WN * 32 * (TN * 32 + 4) * 4;
+  constexpr int BM = WM * TM * MF, BN = WN * TN * MF, MAIN = NS * (BM + BN) * 128, EPI = WM * WN * MF * (TN * MF + 4) * 4;
   constexpr int LDS = MAIN > EPI ? MAIN : EPI;
-  const void* f = reinterpret_cast<const void*>(&token_tile_kernel<T, TM, TN, WM, WN, NS, G, XS, WS>);
+  const void* f = reinterpret_cast<const void*>(&token_tile_kernel<T, MF, TM, TN, WM, WN, NS, G, XS, WS>);
   if (LDS > 65536 && hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return SGA_ERR_HIP;
-  hipLaunchKernelGGL((token_tile_kernel<T, TM, TN, WM, WN, NS, G, XS, WS>), dim3((unsigned)(a.ntm * a.ntn * a.nsplit)), dim3(WM * WN * 64), LDS, st, a);
+  hipLaunchKernelGGL((token_tile_kernel<T, MF, TM, TN, WM, WN, NS, G, XS, WS>), dim3((unsigned)(a.ntm * a.ntn * a.nsplit)), dim3(WM * WN * 64), LDS, st, a);
   LAUNCHED();
   return SGA_OK;
 }
 template <typename T, int G, bool XS, bool WS>
 int run_tile_of(int tile, const TileArgs& a, hipStream_t st) {
   switch (tile) {
-    case 0: return run_tile<T, 2, 4, 4, 2, 2, G, XS, WS>(a, st);
-    case 1: return run_tile<T, 2, 2, 4, 2, 3, G, XS, WS>(a, st);
-    case 2: return run_tile<T, 1, 2, 4, 2, 4, G, XS, WS>(a, st);
-    default: return run_tile<T, 1, 1, 2, 2, 4, G, XS, WS>(a, st);
+    case 0: return run_tile<T, 32, 2, 4, 4, 2, 2, G, XS, WS>(a, st);
+    case 1: return run_tile<T, 32, 2, 2, 4, 2, 3, G, XS, WS>(a, st);
+    case 2: return run_tile<T, 32, 1, 2, 4, 2, 4, G, XS, WS>(a, st);
+    case 3:
+      if constexpr (!XS) return run_tile<T, 16, 3, 2, 2, 2, 4, G, XS, WS>(a, st);
+      return SGA_ERR_UNSUPPORTED;      // 96 rows of a strided X: make_plan takes another tile
+    default: return run_tile<T, 32, 1, 1, 2, 2, 4, G, XS, WS>(a, st);
   }
 }
 template <typename T, int G>
