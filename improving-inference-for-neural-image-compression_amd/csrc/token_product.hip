@@ -8,7 +8,8 @@
 //               ds_read_b32 (32 bit)
 // with the 16-byte pieces of a row permuted by the row index (the lanes of the DMA fetch permuted addresses: LDS-DMA writes lane
 // after lane), so that the fragment reads of a wave spread over all banks.  Rows past M or N repeat the last one (not stored),
-// pieces past K are out of the buffer descriptor's range and arrive as zeros.
+// pieces past K are out of the buffer descriptor's range and arrive as zeros; the one that
+// K ends in comes through registers.
 //
 // The product is taken as W X^T per wave (MFMA rows = n, columns = m): a lane then holds 4 adjacent n of one m.  Results pass
 // through LDS once more (32 rows of f32 per wave) so that every lane stores 8 adjacent columns, with bias, activation,
@@ -91,7 +92,8 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(
 constexpr uint32_t kOutside = 0x80000000u;      // = num_records: a lane with this offset reads zeros
 
 // One operand's tile of R rows (m or n) per K step: how it is fetched and how its fragments are read.  G: bytes that a lane fetches at
-// a time, 16, or 4 where rows are not made of aligned 16-byte pieces (then with four times the instructions)
+// a time, 16, or 4 where the rows of a strided operand are not made of 16-byte pieces (then with four times the instructions).  The
+// addresses are multiples of 4.
 template <typename T, int R, bool S, int NT, int G, int MF>
 struct Side {
   static constexpr int E = sizeof(T), KS = 128 / E, PASSES = R * 128 / (NT * G);      // KS: k per step
@@ -148,7 +150,7 @@ struct Side {
     }
   }
   // the next step's tile: open, then one piece after the other into LDS at `lds`; left: what of K there is from the step's start on, in
-  // bytes (adjacent) or rows (strided), 0 or less: nothing
+  // bytes (adjacent; a piece that is not whole is left out) or rows (strided), 0 or less: nothing
   __device__ __forceinline__ void open() {
     const uint64_t b = (uint64_t)base;
     srd[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
@@ -158,7 +160,7 @@ struct Side {
     base += step;
   }
   __device__ __forceinline__ void piece(int i, uint32_t lds, int left) {
-    const uint32_t v = kpos_of(i) < left ? voff[i] : kOutside;
+    const uint32_t v = (S ? kpos_of(i) < left : kpos_of(i) + G <= left) ? voff[i] : kOutside;
     if constexpr (G == 16) dma16(lds + i * NT * 16, v, srd);
     else dma4(lds + i * NT * 4, v, srd);
   }
@@ -264,6 +266,30 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void token_tile_kernel(const TileA
   // not used (fetches out of range leave zeros).
   constexpr int P = PX + PW, NG = MF / 8, Q = NS == 2 ? P : (P + NG - 1) / NG;      // fetches in a group
   constexpr auto upto = [](int g) { return g * Q < P ? g * Q : P; };
+  // K adjacent and no multiple of 16 bytes: the last piece of each row, which the fetches leave out, comes element by element
+  // through registers, one row per lane; its elements past K are zeros
+  static_assert(NT >= BM + BN, "a row per lane");
+  constexpr int V = 16 / (int)sizeof(T);
+  const int row = threadIdx.x, odd = (int)(a.K % V);
+  const bool ragged = odd != 0 && k1 == a.nk && !(XS && WS);
+  u32x4 tail = {0, 0, 0, 0};
+  char* tail_to = nullptr;
+  if (ragged && (row < BM ? !XS : row < BM + BN && !WS)) {
+    const int r = row < BM ? row : row - BM;
+    const int64_t at = row < BM ? (m0 + r < a.M ? m0 + r : a.M - 1) * a.ld_x : (n0 + r < a.N ? n0 + r : a.N - 1) * a.ld_w;
+    const T* from = (const T*)((row < BM ? a.x : a.w) + at) + (a.K - odd);
+    T v[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = j < odd ? from[j] : (T)0.f;
+    __builtin_memcpy(&tail, v, 16);
+    const int chunk = (int)((a.K - odd) * (int64_t)sizeof(T) % 128) >> 4;
+    if constexpr (!XS) { if (row < BM) tail_to = smem + r * 128 + (X::slot_of(chunk, r) << 4); }
+    if constexpr (!WS) { if (row >= BM) tail_to = smem + BM * 128 + r * 128 + (W::slot_of(chunk, r) << 4); }
+  }
+  auto add_tail = [&](int stage) {
+    if (tail_to) *(u32x4*)(tail_to + stage * STAGE) = tail;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
   if (k1 > k0) {
 #pragma unroll 1
     for (int st = 0; st < NS - 1; ++st) {
@@ -276,6 +302,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void token_tile_kernel(const TileA
 #pragma unroll
     for (int f = 0; f < Q; ++f) piece(f, NS - 1);
     barrier_but<(NS - 2) * P + Q>();
+    if (ragged && k1 - k0 == 1) add_tail(0);
 #pragma unroll
     for (int f = 0; f < TM + TN; ++f) read(0, 0, 0, f);
     int stage = 0, prev = NS - 1;
@@ -285,6 +312,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void token_tile_kernel(const TileA
 #pragma unroll
       for (int g = 0; g < NG - 1; ++g) group(g & 1, stage, g + 1, upto(g + 1), upto(g + 2), prev);
       barrier_but<(NS - 2) * P>();
+      if (ragged && k == k1 - 2) add_tail(next);
       k_left -= X::KS;
       open();
       group((NG - 1) & 1, next, 0, 0, upto(1), stage);
@@ -478,14 +506,14 @@ struct Plan {
   int64_t x_off, w_off, part_off, bytes, ld_part;
 };
 
-// bytes that a lane can fetch at a time: all along rows of aligned pieces of 16, or of 4; 0: the operand has to be copied first.  A
-// tile's rows have to lie within the 2 GiB that an offset of the buffer descriptor spans.
-int fetch_bytes(const Operand& o, int64_t rows, int64_t K, int E) {
-  const int64_t inner = o.strided ? rows : K, outer = o.strided ? 128 / E : 256;
-  if (outer * o.ld * E >= (1ll << 31) - 65536) return 0;
-  const uint64_t bits = (uint64_t)(uintptr_t)o.p | (uint64_t)(o.ld * E);
-  if (!(bits & 15) && (o.padded || (inner * E) % 16 == 0)) return 16;
-  return !(bits & 3) && (o.padded || (inner * E) % 4 == 0) ? 4 : 0;
+// bytes that a lane can fetch at a time, 0: the operand has to be copied first.  Pieces of 16 need rows that start at multiples of 4
+// bytes, and for a strided operand rows of whole pieces (what is past K is made up by the kernel, what is past M or N would
+// be past the operand's end).  A tile's rows have to lie within the 2 GiB that an offset of the buffer descriptor spans.
+int fetch_bytes(const Operand& o, int64_t rows, int E) {
+  if ((o.strided ? 128 / E : 256) * o.ld * E >= (1ll << 31) - 65536) return 0;
+  if (((uint64_t)(uintptr_t)o.p | (uint64_t)(o.ld * E)) & 3) return 0;
+  if (!o.strided || o.padded || (rows * E) % 16 == 0) return 16;
+  return (rows * E) % 4 == 0 ? 4 : 0;
 }
 
 // tile, workgroups that are resident at a time, and the times of a K step and of everything else in a tile's life, in ns
@@ -502,7 +530,7 @@ Plan make_plan(const Product& p) {
     o.few = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
     return o;
   }
-  const int gx = fetch_bytes(p.x, p.M, p.K, E), gw = fetch_bytes(p.w, p.N, p.K, E);
+  const int gx = fetch_bytes(p.x, p.M, E), gw = fetch_bytes(p.w, p.N, E);
   o.pack_x = gx == 0;
   o.pack_w = gw == 0;
   o.fetch = gx == 4 || gw == 4 ? 4 : 16;
@@ -549,7 +577,7 @@ int run_tile_of(int tile, const TileArgs& a, hipStream_t st) {
 }
 template <typename T, int G>
 int run_order(int tile, bool xs, bool ws, const TileArgs& a, hipStream_t st) {
-  if (!xs && !ws) return run_tile_of<T, G, false, false>(tile, a, st);
+  if constexpr (G == 16) { if (!xs && !ws) return run_tile_of<T, G, false, false>(tile, a, st); }
   if (!xs) return run_tile_of<T, G, false, true>(tile, a, st);
   return run_tile_of<T, G, true, true>(tile, a, st);
 }
