@@ -172,15 +172,26 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float v
   *(t8*)p = a;
 }
 
+// The residual is loaded apart from the rest (residual8), so that a lane can have several rows' on their way: the
+// compiler may not move a load before a store to `out`, which may be the same tensor.
+template <typename T> struct Raw8 { u32x4 q[sizeof(T) / 2]; };      // 8 elements as they lie
+template <typename T>
+__device__ __forceinline__ Raw8<T> residual8(const Epilogue& e, int64_t m, int64_t n) {
+  Raw8<T> r = {};
+  if (e.residual) r = *(const Raw8<T>*)((const T*)e.residual + m * e.ld_residual + n);
+  return r;
+}
+template <typename T> __device__ __forceinline__ void bias8(const Epilogue& e, int64_t n, float b[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) b[j] = 0.f;
+  if (e.bias) load8((const T*)e.bias + n, b);
+}
 // columns n .. n + 7 of row m, all of them there and aligned (e.vec); seed / offset: drop_key's
 template <typename T>
-__device__ __forceinline__ void epilogue8(const Epilogue& e, uint64_t seed, uint64_t offset, int64_t m, int64_t n, float v[8]) {
-  if (e.bias) {
-    float b[8];
-    load8((const T*)e.bias + n, b);
+__device__ __forceinline__ void epilogue8(const Epilogue& e, uint64_t seed, uint64_t offset, int64_t m, int64_t n, float v[8], const float b[8],
+                                          const Raw8<T>& res) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] += b[j];
-  }
+  for (int j = 0; j < 8; ++j) v[j] += b[j];
   if (e.pre) store8((T*)e.pre + m * e.cols + n, v);
   act_values<8>(v, e.act);
   if (e.drop.on) {
@@ -192,22 +203,45 @@ __device__ __forceinline__ void epilogue8(const Epilogue& e, uint64_t seed, uint
     for (int j = 0; j < 8; ++j) v[j] = drop_apply(e.drop, w[j], v[j]);
   }
   if (e.residual) {
-    float r[8];
-    load8((const T*)e.residual + m * e.ld_residual + n, r);
+    T r[8];
+    __builtin_memcpy(r, &res, sizeof(r));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] += r[j];
+    for (int j = 0; j < 8; ++j) v[j] += to_f32(r[j]);
   }
   store8((T*)e.out + m * e.ld_out + n, v);
 }
-// one element, of any row length and alignment: lanes take neighbouring columns
-template <typename T>
-__device__ __forceinline__ void epilogue1(const Epilogue& e, uint64_t seed, uint64_t offset, int64_t m, int64_t n, float u) {
-  if (e.bias) u += to_f32(((const T*)e.bias)[n]);
-  if (e.pre) ((T*)e.pre)[m * e.cols + n] = from_f32<T>(u);
-  act_values<1>(&u, e.act);
-  if (e.drop.on) u = drop_one(e.drop, seed, offset, (uint64_t)(m * e.cols + n), u);
-  if (e.residual) u += to_f32(((const T*)e.residual)[m * e.ld_residual + n]);
-  ((T*)e.out)[m * e.ld_out + n] = from_f32<T>(u);
+// N elements (m[j], n[j]) of any row length and alignment: lanes take neighbouring columns.  live: bit j = it exists
+__device__ __noinline__ inline uint32_t drop_word(uint64_t seed, uint64_t offset, uint64_t i) {
+  uint32_t w[4];
+  drop_words(seed, offset, i >> 2, w);
+  const int j = (int)(i & 3);
+  return j == 0 ? w[0] : j == 1 ? w[1] : j == 2 ? w[2] : w[3];
+}
+template <typename T, int N>
+__device__ __forceinline__ void epilogue1(const Epilogue& e, uint64_t seed, uint64_t offset, const int64_t m[N], const int64_t n[N], unsigned live,
+                                          float u[N]) {
+  float res[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    res[j] = 0.f;
+    if (live >> j & 1) {
+      if (e.residual) res[j] = to_f32(((const T*)e.residual)[m[j] * e.ld_residual + n[j]]);
+      if (e.bias) u[j] += to_f32(((const T*)e.bias)[n[j]]);
+    }
+  }
+  if (e.pre) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (live >> j & 1) ((T*)e.pre)[m[j] * e.cols + n[j]] = from_f32<T>(u[j]);
+  }
+  act_values<N>(u, e.act);
+  if (e.drop.on) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) u[j] = drop_apply(e.drop, drop_word(seed, offset, (uint64_t)(m[j] * e.cols + n[j])), u[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (live >> j & 1) ((T*)e.out)[m[j] * e.ld_out + n[j]] = from_f32<T>(e.residual ? u[j] + res[j] : u[j]);
 }
 
 // ---- C[m, n] = epilogue(sum_k X(m, k) W(n, k)) (token_product.hip) -------------------------------------------------------

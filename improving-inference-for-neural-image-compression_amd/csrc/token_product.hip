@@ -329,7 +329,11 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void token_tile_kernel(const TileA
   const int lane = threadIdx.x & 63;
   uint64_t seed = 0, offset = 0;
   if (a.e.drop.on) drop_key(a.e.drop, seed, offset);
-  constexpr int COLS = TN * MF, LPR = COLS / 8;      // lanes per row of 8-column pieces
+  constexpr int COLS = TN * MF, LPR = COLS / 8, RPP = 64 / LPR;      // lanes per row of 8-column pieces, rows per pass
+  static_assert(MF % RPP == 0 && MF * COLS % 512 == 0, "whole passes");
+  const int64_t np = n0 + wn + (lane % LPR) * 8;
+  float b8[8] = {};
+  if (a.e.vec && np < a.N) bias8<T>(a.e, np, b8);
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
 #pragma unroll
@@ -339,22 +343,42 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void token_tile_kernel(const TileA
         *(f32x4*)(sh + (lane % MF) * PITCH + j * MF + c * 8 + (lane / MF) * 4) =
             f32x4{acc[i][j][0][c * 4], acc[i][j][0][c * 4 + 1], acc[i][j][0][c * 4 + 2], acc[i][j][0][c * 4 + 3]};
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the rows below are other lanes' writes of this wave
-    if (a.e.vec || a.nsplit > 1) {
+    const int64_t mi = m0 + wm + i * MF;
+    if (a.nsplit > 1) {
+      float* to = a.part + ((int64_t)z * a.M + mi) * a.ld_part + np;
 #pragma unroll 1
-      for (int r = lane / LPR; r < MF; r += 64 / LPR) {
+      for (int r = lane / LPR; r < MF; r += RPP) {
         float v[8];
         load8(sh + r * PITCH + (lane % LPR) * 8, v);
-        const int64_t m = m0 + wm + i * MF + r, n = n0 + wn + (lane % LPR) * 8;
-        if (m >= a.M || n >= a.N) continue;
-        if (a.nsplit > 1) store8(a.part + ((int64_t)z * a.M + m) * a.ld_part + n, v);
-        else epilogue8<T>(a.e, seed, offset, m, n, v);
+        if (mi + r < a.M && np < a.N) store8(to + r * a.ld_part, v);
+      }
+    } else if (a.e.vec) {
+      Raw8<T> res = {}, next = {};      // the next row's residual is on its way while this row is worked on
+      int r = lane / LPR;
+      if (mi + r < a.M && np < a.N) res = residual8<T>(a.e, mi + r, np);
+#pragma unroll 1
+      for (; r < MF; r += RPP) {
+        if (r + RPP < MF && mi + r + RPP < a.M && np < a.N) next = residual8<T>(a.e, mi + r + RPP, np);
+        float v[8];
+        load8(sh + r * PITCH + (lane % LPR) * 8, v);
+        if (mi + r < a.M && np < a.N) epilogue8<T>(a.e, seed, offset, mi + r, np, v, b8, res);
+        res = next;
       }
     } else {
-#pragma unroll 4
-      for (int r = 0; r < MF * COLS / 64; ++r) {
-        const int at = r * 64 + lane, row = at / COLS, col = at % COLS;
-        const int64_t m = m0 + wm + i * MF + row, n = n0 + wn + col;
-        if (m < a.M && n < a.N) epilogue1<T>(a.e, seed, offset, m, n, sh[row * PITCH + col]);
+#pragma unroll 1
+      for (int r0 = 0; r0 < MF * COLS / 64; r0 += 8) {
+        int64_t m[8], n[8];
+        float u[8];
+        unsigned live = 0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int at = (r0 + q) * 64 + lane;
+          m[q] = mi + at / COLS;
+          n[q] = n0 + wn + at % COLS;
+          if (m[q] < a.M && n[q] < a.N) live |= 1u << q;
+          u[q] = sh[at / COLS * PITCH + at % COLS];
+        }
+        epilogue1<T, 8>(a.e, seed, offset, m, n, live, u);
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -399,6 +423,15 @@ __global__ __launch_bounds__(512, 1) void token_few_kernel(const FewArgs a) {
   const char* wrow = a.w + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ld_w;
 #pragma unroll
   for (int i = 0; i < MB; ++i) xrow[i] = a.x + (i * 16 + r < a.M ? i * 16 + r : a.M - 1) * a.ld_x;
+  // what the last lines need besides the sums is fetched under them
+  const int mo = threadIdx.x >> 1;
+  const int64_t no = n0 + (threadIdx.x & 1) * 8;
+  float b8[8] = {};
+  Raw8<T> res = {};
+  if (a.e.vec && mo < a.M && no < a.N) {
+    bias8<T>(a.e, no, b8);
+    res = residual8<T>(a.e, mo, no);
+  }
   f32x4 acc[MB];
 #pragma unroll
   for (int i = 0; i < MB; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -439,15 +472,15 @@ __global__ __launch_bounds__(512, 1) void token_few_kernel(const FewArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += u[j];
     }
-    epilogue8<T>(a.e, seed, offset, m, n0 + c, v);
+    epilogue8<T>(a.e, seed, offset, m, n0 + c, v, b8, res);
   } else {
     for (int i = threadIdx.x; i < MB * 256; i += 512) {
-      const int m = i >> 4, c = i & 15;
-      if (m >= a.M || n0 + c >= a.N) continue;
-      float v = sh[0][m][c];
+      const int64_t m = i >> 4, n = n0 + (i & 15);
+      if (m >= a.M || n >= a.N) continue;
+      float v = sh[0][m][i & 15];
 #pragma unroll
-      for (int s = 1; s < 8; ++s) v += sh[s][m][c];
-      epilogue1<T>(a.e, seed, offset, m, n0 + c, v);
+      for (int s = 1; s < 8; ++s) v += sh[s][m][i & 15];
+      epilogue1<T, 1>(a.e, seed, offset, &m, &n, 1, &v);
     }
   }
 }
@@ -463,17 +496,20 @@ __global__ __launch_bounds__(256) void token_join_kernel(const float* __restrict
   const float* p = part + m * ld_part + n;
   if constexpr (VEC) {
     float v[8], u[8];
+    float b[8];
+    bias8<T>(e, n, b);
+    const Raw8<T> res = residual8<T>(e, m, n);
     load8(p, v);
     for (int s = 1; s < nsplit; ++s) {
       load8(p + s * M * ld_part, u);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += u[j];
     }
-    epilogue8<T>(e, seed, offset, m, n, v);
+    epilogue8<T>(e, seed, offset, m, n, v, b, res);
   } else {
     float v = *p;
     for (int s = 1; s < nsplit; ++s) v += p[s * M * ld_part];
-    epilogue1<T>(e, seed, offset, m, n, v);
+    epilogue1<T, 1>(e, seed, offset, &m, &n, 1, &v);
   }
 }
 
