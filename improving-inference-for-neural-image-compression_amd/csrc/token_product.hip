@@ -552,10 +552,17 @@ int fetch_bytes(const Operand& o, int64_t rows, int E) {
   return (rows * E) % 4 == 0 ? 4 : 0;
 }
 
-// tile, workgroups that are resident at a time, and the times of a K step and of everything else in a tile's life, in ns
-struct Tile { int m, n, slots; double step16, step32, once; };
+// The tiles and what they cost, measured over 20 shapes from 32 x 4096 x 4096 to 8192 x 16384 x 4096 (128 to 8192 workgroups, K splits 1
+// to 8; the plan found is within 6 % of the fastest there): ns of a K step of a workgroup with 1 and with 2 of them on its CU (as
+// many as the LDS holds), 16- and 32-bit types, and of the rest of a tile's life.
+struct Tile { int m, n, per_cu; double step[2][2], once; };
 constexpr int kTiles = 5;
-const Tile kTile[kTiles] = {{256, 256, 256, 1650, 14500, 11000}, {256, 128, 256, 1050, 7600, 8000}, {128, 128, 256, 620, 4000, 5000}, {96, 64, 512, 600, 2500, 3000}, {64, 64, 512, 500, 1900, 3000}};
+const Tile kTile[kTiles] = {{256, 256, 1, {{1600, 0}, {7350, 0}}, 9000},
+                            {256, 128, 1, {{930, 0}, {3800, 0}}, 5000},
+                            {128, 128, 1, {{560, 0}, {1960, 0}}, 3500},
+                            {96, 64, 2, {{300, 470}, {880, 1500}}, 3000},
+                            {64, 64, 2, {{270, 410}, {620, 1090}}, 2500}};
+constexpr int kCUs = 256;
 
 Plan make_plan(const Product& p) {
   const int E = (int)dtype_bytes(p.dtype), V = 16 / E;
@@ -573,15 +580,23 @@ Plan make_plan(const Product& p) {
   if (o.pack_x) { o.ldp_x = round_up(p.x.strided ? p.M : p.K, V); o.x_off = o.bytes; o.bytes += round_up((p.x.strided ? p.K : p.M) * o.ldp_x * E, 256); }
   if (o.pack_w) { o.ldp_w = round_up(p.w.strided ? p.N : p.K, V); o.w_off = o.bytes; o.bytes += round_up((p.w.strided ? p.K : p.N) * o.ldp_w * E, 256); }
   const int64_t nk = ceil_div(p.K, 128 / E);
+  // rows off the 16-byte grid cost a lone workgroup a fifth more per step (two on a CU cover it for each other); results that leave
+  // element by element, 4 us more at the end of a tile, which the join's many small workgroups do not feel
+  const bool off = o.fetch == 4 || (((uint64_t)(uintptr_t)p.x.p | (uint64_t)(p.x.ld * E) | (uint64_t)(uintptr_t)p.w.p | (uint64_t)(p.w.ld * E)) & 15);
   double best = 1e300;
   o.nsplit = 1;
   for (int t = 0; t < kTiles; ++t) {
     if (kTile[t].m == 96 && p.x.strided) continue;      // the keys of a k row need a power of two
     const int64_t tiles = ceil_div(p.M, kTile[t].m) * ceil_div(p.N, kTile[t].n);
+    const Tile& c = kTile[t];
+    const double* step = c.step[E == 4];
     for (int s = 1; s == 1 || (s <= 16 && s <= nk); ++s) {
-      const double rounds = (double)ceil_div(tiles * s, kTile[t].slots);
-      double cost = rounds * ((double)ceil_div(nk, s) * (E == 4 ? kTile[t].step32 : kTile[t].step16) + kTile[t].once);
-      if (s > 1) cost += 4000.0 + (double)p.M * p.N * (s * 8.0 + E) / 3500.0;      // the slabs' way out and back at 3.5 TB/s, a launch
+      const int64_t at_once = (int64_t)kCUs * c.per_cu, rest = tiles * s % at_once;
+      const double steps = (double)ceil_div(nk, s);
+      double cost = (double)(tiles * s / at_once) * (steps * step[c.per_cu - 1] + c.once);
+      if (rest) cost += steps * step[rest > kCUs] * (off && rest <= kCUs ? 1.2 : 1.0) + c.once;
+      if (s == 1 && !p.e.vec) cost += 4000.0;
+      if (s > 1) cost += 3000.0 + (double)p.M * p.N * (s * 8.0 + E) / 4000.0;      // a launch, the slabs' way out and back at 4 TB/s
       if (cost < best) { best = cost; o.tile = t; o.nsplit = s; }
     }
   }
