@@ -33,6 +33,7 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _U64 = (1 << 64) - 1
 _Tensor = torch.Tensor
 _empty = torch.empty
+_empty_like = torch.empty_like
 
 # The argument structures as bytes: a call is a few microseconds long, and filling a ctypes structure would be half of it.
 _DROP = "dQQP"
@@ -87,11 +88,18 @@ def _rows_of_any(t, what, dtype, device, features):
 def _vector(t, what, n, dtypes, device):
     if t is None:
         return 0
+    if isinstance(t, _Tensor) and t.dtype in dtypes and t.shape == (n,) and t.is_contiguous() and t.device == device:
+        return t.data_ptr()
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
         raise TypeError("%s: a tensor of %s is expected" % (what, " or ".join(str(d) for d in dtypes)))
     if t.device != device or tuple(t.shape) != (n,) or not t.is_contiguous():
         raise ValueError("%s: %d adjacent values on %s are expected, got %s on %s" % (what, n, device, tuple(t.shape), t.device))
     return t.data_ptr()
+
+
+def _like(x):
+    """A tensor for a result of x's shape and type (rows without gaps)."""
+    return _empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
 
 
 def _same(t, like, what):
@@ -172,12 +180,12 @@ def linear(x, weight, bias=None, act="none", residual=None, dropout=None, want_p
         _same(residual, shape, "residual")
         p_res = residual.data_ptr()
     if out is None:
-        out = _empty(shape, dtype=dt, device=dev)
+        out = x.new_empty(shape)
     else:
         _, _, ld_out = _rows(out, "out", dt, dev, n)
         _same(out, shape, "out")
     if want_pre:
-        pre = _empty(shape, dtype=dt, device=dev)
+        pre = x.new_empty(shape)
         p_pre = pre.data_ptr()
     a = _LINEAR(rows, k, n, _DTYPES[dt], _act(act), x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _vector(bias, "bias", n, (dt,), dev), p_res, ld_res,
                 out.data_ptr(), ld_out, p_pre, 0, 0, 0, 0, 0, *_drop(dropout, dev))
@@ -201,7 +209,7 @@ def linear_grad(g_out, x, weight, pre=None, act="none", dropout=None, want=(True
         _rows(pre, "pre", dt, dev, n)
         _same(pre, g_out.shape, "pre")
         _contiguous(pre, "pre")
-    g_x = _empty(x.shape, dtype=dt, device=dev) if want[0] else None
+    g_x = _like(x) if want[0] else None
     g_w = _empty((n, k), dtype=dt, device=dev) if want[1] else None
     g_b = _empty(n, dtype=dt, device=dev) if want[2] else None
     a = _LINEAR(rows, k, n, _DTYPES[dt], code, x.data_ptr(), ld_x, weight.data_ptr(), ld_w, 0, 0, 0, 0, 0, pre.data_ptr() if code else 0,
@@ -221,10 +229,12 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, want_stats=False):
     w, b = _vector(weight, "weight", n, (dt, torch.float32), dev), _vector(bias, "bias", n, (pt,), dev)
     if not eps >= 0.0:
         raise ValueError("eps: a number >= 0 is expected, got %r" % (eps,))
-    y = _empty(x.shape, dtype=dt, device=dev)
+    y = _like(x)
+    mean = rstd = None
     p_mean = p_rstd = 0
     if want_stats:
-        mean, rstd = _empty(x.shape[:-1], dtype=torch.float32, device=dev), _empty(x.shape[:-1], dtype=torch.float32, device=dev)
+        mean = _empty(x.shape[:-1], dtype=torch.float32, device=dev)
+        rstd = _empty_like(mean)
         p_mean, p_rstd = mean.data_ptr(), rstd.data_ptr()
     st = _call("sga_op_layer_norm_fwd", dev, _NORM(rows, n, _DTYPES[dt], _DTYPES[pt], eps, x.data_ptr(), ld, w, b, y.data_ptr(), p_mean, p_rstd,
                                                    0, 0, 0, 0, 0, 0, 0))
@@ -252,7 +262,7 @@ def layer_norm_grad(g_y, x, mean, rstd, weight=None, g_add=None, want=(True, Tru
     pt = weight.dtype if weight is not None else param_dtype or dt
     if pt not in (dt, torch.float32):
         raise TypeError("param_dtype: %s or torch.float32 is expected, got %s" % (dt, pt))
-    g_x = _empty(x.shape, dtype=dt, device=dev) if want[0] else None
+    g_x = _like(x) if want[0] else None
     g_w = _empty(n, dtype=pt, device=dev) if want[1] else None
     g_b = _empty(n, dtype=pt, device=dev) if want[2] else None
     a = _NORM(rows, n, _DTYPES[dt], _DTYPES[pt], 0.0, x.data_ptr(), ld, w, 0, 0, mean.data_ptr(), rstd.data_ptr(), g_y.data_ptr(), ld_g,
@@ -272,7 +282,7 @@ def dropout(x, p, seed, offset=0, residual=None):
         _, _, ld_res = _rows(residual, "residual", dt, dev, n)
         _same(residual, x.shape, "residual")
     d = _DROPOUT(*_drop((p, seed) if isinstance(seed, _Tensor) else (p, seed, offset), dev))
-    y = _empty(x.shape, dtype=dt, device=dev)
+    y = _like(x)
     st = _call("sga_op_dropout", dev, x.data_ptr(), ld, residual.data_ptr() if residual is not None else None, ld_res, y.data_ptr(), rows, n,
                _DTYPES[dt], d)
     if st:

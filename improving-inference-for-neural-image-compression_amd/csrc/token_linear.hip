@@ -67,13 +67,24 @@ __global__ __launch_bounds__(256) void token_dz_kernel(const T* __restrict__ g, 
   }
 }
 
+// g_bias = the sum of the partial sums: 32 columns x 8 runs of them per workgroup (a lane per column alone took 35 us for 128 x 8192)
 template <typename T>
 __global__ __launch_bounds__(256) void token_sum_parts_kernel(const float* __restrict__ part, int64_t nparts, T* __restrict__ out, int64_t cols) {
-  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (n >= cols) return;
+  __shared__ float sh[8][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t n = (int64_t)blockIdx.x * 32 + tx, per = (nparts + 7) / 8, p0 = ty * per, p1 = p0 + per < nparts ? p0 + per : nparts;
   float s = 0.f;
-  for (int64_t p = 0; p < nparts; ++p) s += part[p * cols + n];
-  out[n] = from_f32<T>(s);
+  if (n < cols) {
+#pragma unroll 8
+    for (int64_t p = p0; p < p1; ++p) s += part[p * cols + n];
+  }
+  sh[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && n < cols) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += sh[k][tx];
+    out[n] = from_f32<T>(s);
+  }
 }
 
 constexpr int kMaxFeatures = 1 << 20;
@@ -106,7 +117,11 @@ BwdPlan bwd_plan(const sga_linear& a, char* ws) {
   p.dz = (a.act != SGA_ACT_NONE || a.dropout.p > 0.0) && (a.g_x || a.g_w);
   p.part = a.g_bias != nullptr;
   p.ld_dz = round_up(a.out_features, 8);
-  p.per = ceil_div(a.rows, 1024) > 64 ? ceil_div(a.rows, 1024) : 64;      // rows per partial sum of g_bias: at most 1024 of them
+  // rows per workgroup of the dz pass, a partial sum of g_bias each: 64, or as few as 8 where that would leave CUs idle, and at
+  // most 1024 partial sums
+  const int64_t floor = ceil_div(a.rows, 1024), few = a.rows * ceil_div(a.out_features, 256) / 1024 / 8 * 8;
+  p.per = few < 8 ? 8 : few > 64 ? 64 : few;
+  p.per = p.per > floor ? p.per : floor;
   p.chunks = ceil_div(a.rows, p.per);
   if (p.dz) { p.dz_off = p.bytes; p.bytes += round_up(a.rows * p.ld_dz * E, 256); }
   if (p.part) { p.part_off = p.bytes; p.bytes += round_up(p.chunks * a.out_features * 4, 256); }
@@ -175,7 +190,7 @@ int linear_bwd(const sga_linear& a, char* ws, hipStream_t st) {
     LAUNCHED();
   }
   if (p.part) {
-    hipLaunchKernelGGL((token_sum_parts_kernel<T>), dim3((unsigned)ceil_div(a.out_features, 256)), dim3(256), 0, st, part, p.chunks, (T*)a.g_bias,
+    hipLaunchKernelGGL((token_sum_parts_kernel<T>), dim3((unsigned)ceil_div(a.out_features, 32)), dim3(256), 0, st, part, p.chunks, (T*)a.g_bias,
                        (int64_t)a.out_features);
     LAUNCHED();
   }
