@@ -15,7 +15,7 @@ A token is a row: the last dimension holds the features, all others are tokens -
 float32, bfloat16 or float16 tensors of one device; sums and statistics in float32, one rounding on store.  The last dimension has
 stride 1, the dimensions before it one common stride (a slice of a wider buffer, an expanded row); anything else is
 refused, not copied.  Calls run on the current stream of the tensors' device and take their outputs and workspace from torch's
-allocator, so they may be captured into a graph.  `dropout` is (p, seed, offset), or (p, state) with `state` an int64 tensor
+allocator, so they may be captured into a graph; results carry no autograd history.  `dropout` is (p, seed, offset), or (p, state) with `state` an int64 tensor
 {seed, offset} on the device that is read when the kernel runs (a captured graph draws new numbers when it changes).
 There is no CPU path.
 """
@@ -107,6 +107,18 @@ def _same(t, like, what):
         raise ValueError("%s has shape %s, %s is expected" % (what, tuple(t.shape), tuple(like)))
 
 
+def _apart(out, rows, n, ld, t, what, t_rows, t_n, t_ld):
+    """Refuses an output whose memory overlaps an input's; columns side by side in one buffer do not."""
+    if t is None or not rows or not t_rows:
+        return
+    e = out.element_size()
+    a, c = out.data_ptr() // e, t.data_ptr() // e
+    if a < c + (t_rows - 1) * t_ld + t_n and c < a + (rows - 1) * ld + n:
+        side = (a - c) % ld
+        if ld != t_ld or side < t_n or side + n > ld:
+            raise ValueError("out overlaps %s" % what)
+
+
 def _contiguous(t, what):
     if not t.is_contiguous():
         raise ValueError("%s has to be contiguous" % what)
@@ -184,6 +196,13 @@ def linear(x, weight, bias=None, act="none", residual=None, dropout=None, want_p
     else:
         _, _, ld_out = _rows(out, "out", dt, dev, n)
         _same(out, shape, "out")
+        if ld_out == 0 and rows > 1:
+            raise ValueError("out: its rows overlap")
+        _apart(out, rows, n, ld_out, x, "x", rows, k, ld_x)
+        _apart(out, rows, n, ld_out, weight, "weight", n, k, ld_w)
+        _apart(out, rows, n, ld_out, bias, "bias", 1, n, n)
+        if p_res != out.data_ptr() or ld_res != ld_out:
+            _apart(out, rows, n, ld_out, residual, "residual", rows, n, ld_res)
     if want_pre:
         pre = x.new_empty(shape)
         p_pre = pre.data_ptr()

@@ -19,69 +19,82 @@ template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T
 
 // e^x to 2 units in the last place: 2^(x log2 e) by the hardware's exp2, and the part of x log2 e that float32 cannot hold as a
 // factor.  The clamp keeps infinities out of that part; a NaN becomes some number, every use multiplies by x again.
-__device__ __forceinline__ float exp_f(float x) {
+// SHORT (results of 16 bits, whose half step is 2^-12 at the least): without that part, off by |x| 2^-24.
+template <bool SHORT> __device__ __forceinline__ float exp_f(float x) {
+  if constexpr (SHORT) return __builtin_amdgcn_exp2f(x * 1.44269504f);
   x = fminf(fmaxf(x, -1000.f), 1000.f);
   const float t = x * 1.44269504f;
   const float e = fmaf(x, 1.925963033e-8f, fmaf(x, 1.44269504f, -t));
   return __builtin_amdgcn_exp2f(t) * fmaf(e, 0.69314718f, 1.f);
 }
-// 1 / (1 + e^-x)
-__device__ __forceinline__ float sigmoid_f(float x) { return __builtin_amdgcn_rcpf(1.f + exp_f(-x)); }
 
-// Phi(-|z|) = erfc(|z| / sqrt 2) / 2 = g(|z|) e^(-z^2 / 2) with g smooth and slowly varying: g as a polynomial of degree 8 in
-// t = 1 / (1 + 0.3 |z|), fitted on 0 <= |z| <= 14 for the least maximum of the relative error (5.8e-8 in exact arithmetic, 5e-7 with
-// float32 steps; beyond 14 the exponential is 0).  Relative accuracy in the tail is what 1 + erf(z) cannot give, and the
-// backward pass shares the exponential: 8 + 10 instructions where the library's erf and exp take about 60.
-__device__ __forceinline__ float normal_tail(float z, float gauss) {
+// Phi(-|z|) = erfc(|z| / sqrt 2) / 2 = g(|z|) e^(-z^2 / 2) with g smooth and slowly varying: g as a polynomial in t = 1 / (1 + 0.3 |z|),
+// fitted on 0 <= |z| <= 14 for the least maximum of the relative error (beyond, the exponential is 0): degree 8 is off by 5.8e-8 in
+// exact arithmetic, 5e-7 with float32 steps; degree 6, for SHORT results, by 1.9e-6.  Relative accuracy in the tail is what
+// 1 + erf(z) cannot give, and the backward pass shares the exponential: about 25 (SHORT: 18) instructions where the
+// library's erf and exp take about 60.
+template <bool SHORT> __device__ __forceinline__ float normal_tail(float z, float gauss) {
   const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.3f, 1.f));
-  float p = 0.038378264755010605f;
-  p = fmaf(p, t, -0.16916599869728088f);
-  p = fmaf(p, t, 0.22865986824035645f);
-  p = fmaf(p, t, -0.07650627195835114f);
-  p = fmaf(p, t, 0.14253540337085724f);
-  p = fmaf(p, t, 0.09468357264995575f);
-  p = fmaf(p, t, 0.12192033231258392f);
-  p = fmaf(p, t, 0.1194876879453659f);
-  p = fmaf(p, t, 7.168815500335768e-06f);
+  float p;
+  if constexpr (SHORT) {
+    p = -0.08459318429231644f;
+    p = fmaf(p, t, 0.24057263135910034f);
+    p = fmaf(p, t, -0.04864419996738434f);
+    p = fmaf(p, t, 0.16476432979106903f);
+    p = fmaf(p, t, 0.10670459270477295f);
+    p = fmaf(p, t, 0.1212746873497963f);
+    p = fmaf(p, t, -7.978831126820296e-05f);
+  } else {
+    p = 0.038378264755010605f;
+    p = fmaf(p, t, -0.16916599869728088f);
+    p = fmaf(p, t, 0.22865986824035645f);
+    p = fmaf(p, t, -0.07650627195835114f);
+    p = fmaf(p, t, 0.14253540337085724f);
+    p = fmaf(p, t, 0.09468357264995575f);
+    p = fmaf(p, t, 0.12192033231258392f);
+    p = fmaf(p, t, 0.1194876879453659f);
+    p = fmaf(p, t, 7.168815500335768e-06f);
+  }
   return p * gauss;
 }
 
-template <int ACT> __device__ __forceinline__ float act_value_of(float z) {
+template <int ACT, bool SHORT> __device__ __forceinline__ float act_value_of(float z) {
   if constexpr (ACT == SGA_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
   if constexpr (ACT == SGA_ACT_GELU) {
-    const float q = normal_tail(z, exp_f(-0.5f * z * z));
+    const float q = normal_tail<SHORT>(z, exp_f<SHORT>(-0.5f * z * z));
     return z * (z > 0.f ? 1.f - q : q);
   }
-  if constexpr (ACT == SGA_ACT_GELU_TANH) return z * sigmoid_f(1.59576912160573072f * fmaf(0.044715f * z * z, z, z));
-  if constexpr (ACT == SGA_ACT_SILU) return z * sigmoid_f(z);
+  if constexpr (ACT == SGA_ACT_GELU_TANH)
+    return z * __builtin_amdgcn_rcpf(1.f + exp_f<SHORT>(-1.59576912160573072f * fmaf(0.044715f * z * z, z, z)));
+  if constexpr (ACT == SGA_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + exp_f<SHORT>(-z));
   return z;
 }
-template <int ACT> __device__ __forceinline__ float act_slope_of(float z) {
+template <int ACT, bool SHORT> __device__ __forceinline__ float act_slope_of(float z) {
   if constexpr (ACT == SGA_ACT_RELU) return z > 0.f ? 1.f : 0.f;
   if constexpr (ACT == SGA_ACT_GELU) {
-    const float gauss = exp_f(-0.5f * z * z), q = normal_tail(z, gauss);
+    const float gauss = exp_f<SHORT>(-0.5f * z * z), q = normal_tail<SHORT>(z, gauss);
     return fmaf(z * 0.39894228040143268f, gauss, z > 0.f ? 1.f - q : q);
   }
   if constexpr (ACT == SGA_ACT_GELU_TANH) {
-    const float e = exp_f(-1.59576912160573072f * fmaf(0.044715f * z * z, z, z)), s = __builtin_amdgcn_rcpf(1.f + e);
+    const float e = exp_f<SHORT>(-1.59576912160573072f * fmaf(0.044715f * z * z, z, z)), s = __builtin_amdgcn_rcpf(1.f + e);
     const float c = fminf(fmaxf(z, -16.f), 16.f);      // s (1 - s) is 0 beyond, and the polynomial must not be inf
     const float d = s * (s > 0.f ? e * s : 0.f);       // s (1 - s) without the difference
     return fmaf(c * d, 1.59576912160573072f * fmaf(0.134145f * c, c, 1.f), s) + (z - z);
   }
   if constexpr (ACT == SGA_ACT_SILU) {
-    const float e = exp_f(-z), s = __builtin_amdgcn_rcpf(1.f + e);
+    const float e = exp_f<SHORT>(-z), s = __builtin_amdgcn_rcpf(1.f + e);
     return s > 0.f ? s * fmaf(z, e * s, 1.f) : (z - z);
   }
   return 1.f;
 }
-// v[j] = act(v[j]); g[j] *= act'(v[j])
-template <int N> __device__ __forceinline__ void act_values(float v[N], int act) {
-#define EACH(A) case A: _Pragma("unroll") for (int j = 0; j < N; ++j) v[j] = act_value_of<A>(v[j]); break
+// v[j] = act(v[j]); g[j] *= act'(v[j]);  T: the type of the result
+template <typename T, int N> __device__ __forceinline__ void act_values(float v[N], int act) {
+#define EACH(A) case A: _Pragma("unroll") for (int j = 0; j < N; ++j) v[j] = act_value_of<A, sizeof(T) == 2>(v[j]); break
   switch (act) { EACH(SGA_ACT_RELU); EACH(SGA_ACT_GELU); EACH(SGA_ACT_GELU_TANH); EACH(SGA_ACT_SILU); default: break; }
 #undef EACH
 }
-template <int N> __device__ __forceinline__ void act_slopes(float g[N], const float v[N], int act) {
-#define EACH(A) case A: _Pragma("unroll") for (int j = 0; j < N; ++j) g[j] *= act_slope_of<A>(v[j]); break
+template <typename T, int N> __device__ __forceinline__ void act_slopes(float g[N], const float v[N], int act) {
+#define EACH(A) case A: _Pragma("unroll") for (int j = 0; j < N; ++j) g[j] *= act_slope_of<A, sizeof(T) == 2>(v[j]); break
   switch (act) { EACH(SGA_ACT_RELU); EACH(SGA_ACT_GELU); EACH(SGA_ACT_GELU_TANH); EACH(SGA_ACT_SILU); default: break; }
 #undef EACH
 }
@@ -172,9 +185,37 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float v
   *(t8*)p = a;
 }
 
+// the same past the caches, for streams that nothing on this XCD reads again soon
+template <typename T> __device__ __forceinline__ void load8_once(const T* p, float v[8]) {
+  constexpr int Q = sizeof(T) / 2;
+  u32x4 q[Q];
+#pragma unroll
+  for (int i = 0; i < Q; ++i) q[i] = __builtin_nontemporal_load((const u32x4*)p + i);
+  T t[8];
+  __builtin_memcpy(t, q, sizeof(t));
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = to_f32(t[j]);
+}
+template <typename T> __device__ __forceinline__ void store8_once(T* p, const float v[8]) {
+  constexpr int Q = sizeof(T) / 2;
+  T t[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) t[j] = from_f32<T>(v[j]);
+  u32x4 q[Q];
+  __builtin_memcpy(q, t, sizeof(t));
+#pragma unroll
+  for (int i = 0; i < Q; ++i) __builtin_nontemporal_store(q[i], (u32x4*)p + i);
+}
+
 // The residual is loaded apart from the rest (residual8), so that a lane can have several rows' on their way: the
 // compiler may not move a load before a store to `out`, which may be the same tensor.
 template <typename T> struct Raw8 { u32x4 q[sizeof(T) / 2]; };      // 8 elements as they lie
+template <typename T> __device__ __forceinline__ Raw8<T> raw_once(const T* p) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.q[i] = __builtin_nontemporal_load((const u32x4*)p + i);
+  return r;
+}
 template <typename T>
 __device__ __forceinline__ Raw8<T> residual8(const Epilogue& e, int64_t m, int64_t n) {
   Raw8<T> r = {};
@@ -186,14 +227,17 @@ template <typename T> __device__ __forceinline__ void bias8(const Epilogue& e, i
   for (int j = 0; j < 8; ++j) b[j] = 0.f;
   if (e.bias) load8((const T*)e.bias + n, b);
 }
-// columns n .. n + 7 of row m, all of them there and aligned (e.vec); seed / offset: drop_key's
-template <typename T>
+// columns n .. n + 7 of row m, all of them there and aligned (e.vec); seed / offset: drop_key's.  ONCE: the results bypass the caches
+template <typename T, bool ONCE = false>
 __device__ __forceinline__ void epilogue8(const Epilogue& e, uint64_t seed, uint64_t offset, int64_t m, int64_t n, float v[8], const float b[8],
                                           const Raw8<T>& res) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] += b[j];
-  if (e.pre) store8((T*)e.pre + m * e.cols + n, v);
-  act_values<8>(v, e.act);
+  if (e.pre) {
+    if constexpr (ONCE) store8_once((T*)e.pre + m * e.cols + n, v);
+    else store8((T*)e.pre + m * e.cols + n, v);
+  }
+  act_values<T, 8>(v, e.act);
   if (e.drop.on) {
     const uint64_t g = (uint64_t)(m * e.cols + n) >> 2;      // cols and n are multiples of 8 here
     uint32_t w[8];
@@ -208,7 +252,8 @@ __device__ __forceinline__ void epilogue8(const Epilogue& e, uint64_t seed, uint
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] += to_f32(r[j]);
   }
-  store8((T*)e.out + m * e.ld_out + n, v);
+  if constexpr (ONCE) store8_once((T*)e.out + m * e.ld_out + n, v);
+  else store8((T*)e.out + m * e.ld_out + n, v);
 }
 // N elements (m[j], n[j]) of any row length and alignment: lanes take neighbouring columns.  live: bit j = it exists
 __device__ __noinline__ inline uint32_t drop_word(uint64_t seed, uint64_t offset, uint64_t i) {
@@ -234,7 +279,7 @@ __device__ __forceinline__ void epilogue1(const Epilogue& e, uint64_t seed, uint
     for (int j = 0; j < N; ++j)
       if (live >> j & 1) ((T*)e.pre)[m[j] * e.cols + n[j]] = from_f32<T>(u[j]);
   }
-  act_values<N>(u, e.act);
+  act_values<T, N>(u, e.act);
   if (e.drop.on) {
 #pragma unroll
     for (int j = 0; j < N; ++j) u[j] = drop_apply(e.drop, drop_word(seed, offset, (uint64_t)(m[j] * e.cols + n[j])), u[j]);

@@ -22,7 +22,7 @@ __global__ __launch_bounds__(256) void token_dz_kernel(const T* __restrict__ g, 
   if (d.on) drop_key(d, seed, offset);
   float sum[8] = {};
   for (int64_t m = m0 + py; m < m1 && live > 0; m += 8) {
-    float v[8], z[8];
+    float v[8], z[8] = {};
     if (vec) {
       load8(g + m * ld_g + n, v);
       if (act != SGA_ACT_NONE) load8(pre + m * cols + n, z);
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256) void token_dz_kernel(const T* __restrict__ g, 
         if (d.on) v[j] = j < live ? drop_apply(d, shift == 0 ? w[j] : shift == 1 ? w[j + 1] : shift == 2 ? w[j + 2] : w[j + 3], v[j]) : 0.f;
       }
     }
-    act_slopes<8>(v, z, act);
+    act_slopes<T, 8>(v, z, act);
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum[j] += v[j];
     if (dz) store8(dz + m * ld_dz + n, v);      // ld_dz is a multiple of 8: a ragged last piece ends in zeros

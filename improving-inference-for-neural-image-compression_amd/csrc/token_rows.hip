@@ -69,8 +69,9 @@ __device__ __forceinline__ void row_sum(float (&s)[N], float* sh) {
   }
 }
 
-// y = (x - mean) rstd w + b, mean and variance in two passes over the registers.  Workgroups stay and walk the rows: weights
-// are loaded once, the next row is on its way while this one is summed.
+// y = (x - mean) rstd w + b, mean and variance in two passes over the registers.  Bound by HBM.  Workgroups stay and walk the rows:
+// weights are loaded once, the next row is on its way while this one is summed.  One piece per lane: 16384 x 4096 bf16 (268 MB)
+// 55 us = 4.85 TB/s, against 57 with two pieces on half the lanes and 170 with a workgroup of 256 that reads its row three times.
 template <typename T, typename P, int NT, int L, int V, bool VEC>
 __global__ __launch_bounds__(NT) void layer_norm_fwd_kernel(const T* __restrict__ x, int64_t ld_x, const P* __restrict__ w, const P* __restrict__ b,
                                                             T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd, int64_t rows,
@@ -137,8 +138,10 @@ __global__ __launch_bounds__(NT) void layer_norm_fwd_kernel(const T* __restrict_
 }
 
 // g_x, and this workgroup's share of g_w and g_b: part[block][0][c] = sum of g_y h, part[block][1][c] = sum of g_y over the rows
-// it walks.  The lanes keep their columns' two sums in registers from row to row; the row groups of a workgroup add theirs up
-// in LDS at the end, in a fixed order.
+// it walks.  Bound by HBM: every tensor once.  The lanes keep their columns' two sums and weights in registers from row to row; the
+// row groups of a workgroup add theirs up in LDS at the end, in a fixed order.  8192 x 4096 bf16 with g_add (268 MB): 55 us with the
+// join = 4.9 TB/s; 65 without the weights kept and the streams past the caches (they push the weights out), 70 with 512
+// workgroups (twice the partial sums), 188 as two kernels that read x and g_y twice.
 template <typename T, typename P, int L, int V, bool VEC>
 __global__ __launch_bounds__(1024) void layer_norm_bwd_kernel(const T* __restrict__ x, int64_t ld_x, const P* __restrict__ w,
                                                               const T* __restrict__ gy, int64_t ld_gy, const T* __restrict__ add, int64_t ld_add,
@@ -156,29 +159,75 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_kernel(const T* __restric
 #pragma unroll
     for (int j = 0; j < 8; ++j) sw[v][j] = sb[v][j] = 0.f;
   const int64_t stride = (int64_t)gridDim.x * G, first = (int64_t)blockIdx.x * G;
+  // The next row's pieces are on their way while this row is summed; not so single elements, for odd layouts, and two pieces a
+  // lane, for which the 128 registers of a lane would not do
+  constexpr bool AHEAD = VEC && V == 1;
+  Raw8<T> rx[V] = {}, rg[V] = {}, ra[V] = {};
+  float rmu = 0.f, rr = 0.f;
+  auto ahead = [&](int64_t m) {
+    const int64_t at = m < rows ? m : rows - 1;
+    rmu = mean[at];
+    rr = rstd[at];
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int c = C::at(lane, v, 0);
+        if (c < cols) {
+          rx[v] = raw_once(x + at * ld_x + c);
+          rg[v] = raw_once(gy + at * ld_gy + c);
+          if (add && gx) ra[v] = raw_once(add + at * ld_add + c);
+        }
+      }
+    }
+  };
+  auto weights = [&](int v, float ww[8]) {
+    if constexpr (VEC) {
+      const int c = C::at(lane, v, 0);
+      if (w && c < cols) load8(w + c, ww);
+      else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ww[j] = 1.f;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { const int c = C::at(lane, v, j); ww[j] = w && c < cols ? to_f32(w[c]) : 1.f; }
+    }
+  };
+  float wkept[AHEAD ? V : 1][8];
+  if constexpr (AHEAD) weights(0, wkept[0]);
+  auto open = [](const Raw8<T> (&raw)[V], float (*f)[8]) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      T t[8];
+      __builtin_memcpy(t, &raw[v], sizeof(t));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[v][j] = to_f32(t[j]);
+    }
+  };
+  ahead(first + group);
   int turn = 0;
   for (int64_t m0 = first; m0 < rows; m0 += stride, turn ^= 1) {
     const int64_t m = m0 + group, mr = m < rows ? m : rows - 1;
     const bool live = m < rows;
-    float h[V][8], g[V][8];
-    C::load(x + mr * ld_x, lane, cols, h);
-    C::load(gy + mr * ld_gy, lane, cols, g);
-    const float mu = mean[mr], r = rstd[mr];
+    float h[V][8], g[V][8], a[V][8];
+    const float mu = rmu, r = rr;
+    if constexpr (AHEAD) {
+      open(rx, h);
+      open(rg, g);
+      open(ra, a);
+    } else {
+      C::load(x + mr * ld_x, lane, cols, h);
+      C::load(gy + mr * ld_gy, lane, cols, g);
+    }
+    if (m0 + stride < rows) ahead(m + stride);
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float ww[8];
-      if constexpr (VEC) {
-        const int c = C::at(lane, v, 0);
-        if (w && c < cols) load8(w + c, ww);
-        else {
+      if constexpr (AHEAD) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) ww[j] = 1.f;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) { const int c = C::at(lane, v, j); ww[j] = w && c < cols ? to_f32(w[c]) : 1.f; }
-      }
+        for (int j = 0; j < 8; ++j) ww[j] = wkept[v][j];
+      } else weights(v, ww);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         h[v][j] = C::at(lane, v, j) < cols ? (h[v][j] - mu) * r : 0.f;
@@ -195,19 +244,16 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_kernel(const T* __restric
     row_sum<L, 2>(s, sh[turn]);
     const float c1 = s[0] * inv, c2 = s[1] * inv;
     if (!live) continue;
-    if (add) {
-      float a[V][8];
-      C::load(add + m * ld_add, lane, cols, a);
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g[v][j] = r * (g[v][j] - c1 - h[v][j] * c2) + a[v][j];
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g[v][j] = r * (g[v][j] - c1 - h[v][j] * c2);
+    if constexpr (!AHEAD) {
+      if (add) C::load(add + m * ld_add, lane, cols, a);
     }
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = r * (g[v][j] - c1 - h[v][j] * c2);
+        g[v][j] = add ? d + a[v][j] : d;
+      }
     C::store(gx + m * cols, lane, cols, g);
   }
   if (!part) return;
@@ -346,7 +392,8 @@ __global__ __launch_bounds__(256) void layer_norm_join_kernel(const float* __res
 
 // ---- dropout ---------------------------------------------------------------------------------------------------------------
 // Tensors without gaps, 16-byte aligned: 8 adjacent elements per lane, whatever the row length -- the counter runs over the
-// whole matrix.  The last piece may be short.
+// whole matrix.  The last piece may be short.  Bound by HBM, with the 20 Philox rounds a piece under the loads: 8192 x 8192 bf16 with
+// residual (403 MB) 64 us = 6.3 TB/s (72 through the caches).
 template <typename T, bool RES>
 __global__ __launch_bounds__(256) void dropout_flat_kernel(const T* x, const T* res, T* y, int64_t n, const Drop d) {
   uint64_t seed = 0, offset = 0;
@@ -356,8 +403,8 @@ __global__ __launch_bounds__(256) void dropout_flat_kernel(const T* x, const T* 
     uint32_t w[8];
     float v[8], r[8];
     if (i < pieces) {
-      load8(x + i * 8, v);
-      if constexpr (RES) load8(res + i * 8, r);
+      load8_once(x + i * 8, v);
+      if constexpr (RES) load8_once(res + i * 8, r);
     }
     if (d.on) {
       drop_words(seed, offset, (uint64_t)i * 2, w);
@@ -369,7 +416,7 @@ __global__ __launch_bounds__(256) void dropout_flat_kernel(const T* x, const T* 
         if (d.on) v[j] = drop_apply(d, w[j], v[j]);
         if constexpr (RES) v[j] += r[j];
       }
-      store8(y + i * 8, v);
+      store8_once(y + i * 8, v);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -443,7 +490,7 @@ constexpr int kHeld = 16384;      // the widest row that is held in registers
 
 // Rows of the backward pass are dealt to at most 256 workgroups of 1024 lanes (one per CU): its partial sums of g_w, g_b are 256 x 2
 // rows of float32 then, 3 % of the traffic at 8192 rows.  Long rows: 64 runs of rows.
-int bwd_lanes(int cols) { return cols <= 1024 ? 64 : cols <= 4096 ? 256 : cols <= 8192 ? 512 : 1024; }
+int bwd_lanes(int cols) { return cols <= 512 ? 64 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024; }
 int norm_parts(const sga_layer_norm& a) {
   if (a.rows == 0) return 0;
   const int64_t n = a.cols > kHeld ? a.rows : ceil_div(a.rows, 1024 / bwd_lanes(a.cols));
@@ -477,10 +524,10 @@ int norm_fwd(const sga_layer_norm& a, hipStream_t st) {
   const bool vec = piece_ok(a.x, a.ld_x, a.cols, a.dtype) && piece_ok(a.y, a.cols, a.cols, a.dtype) && piece_ok(a.w, 0, a.cols, a.param_dtype) &&
                    piece_ok(a.b, 0, a.cols, a.param_dtype);
   if (a.cols <= 512) return norm_fwd_held<T, P, 256, 64, 1>(a, vec, st);
-  if (a.cols <= 1024) return norm_fwd_held<T, P, 256, 64, 2>(a, vec, st);
+  if (a.cols <= 1024) return norm_fwd_held<T, P, 256, 128, 1>(a, vec, st);
   if (a.cols <= 2048) return norm_fwd_held<T, P, 256, 256, 1>(a, vec, st);
-  if (a.cols <= 4096) return norm_fwd_held<T, P, 256, 256, 2>(a, vec, st);
-  if (a.cols <= 8192) return norm_fwd_held<T, P, 512, 512, 2>(a, vec, st);
+  if (a.cols <= 4096) return norm_fwd_held<T, P, 512, 512, 1>(a, vec, st);
+  if (a.cols <= 8192) return norm_fwd_held<T, P, 1024, 1024, 1>(a, vec, st);
   if (a.cols <= kHeld) return norm_fwd_held<T, P, 1024, 1024, 2>(a, vec, st);
   hipLaunchKernelGGL((layer_norm_fwd_long_kernel<T, P>), dim3((unsigned)a.rows), dim3(256), 0, st, (const T*)a.x, a.ld_x, (const P*)a.w, (const P*)a.b,
                      (T*)a.y, a.mean, a.rstd, a.cols, a.eps);
@@ -511,10 +558,10 @@ int norm_bwd(const sga_layer_norm& a, float* ws, hipStream_t st) {
                        piece_ok(a.g_add, a.g_add ? a.ld_g_add : 0, a.cols, a.dtype) && piece_ok(a.g_x, a.cols, a.cols, a.dtype) &&
                        piece_ok(a.w, 0, a.cols, a.param_dtype);
       if (a.cols <= 512) s = norm_bwd_held<T, P, 64, 1>(a, vec, part, np, st);
-      else if (a.cols <= 1024) s = norm_bwd_held<T, P, 64, 2>(a, vec, part, np, st);
+      else if (a.cols <= 1024) s = norm_bwd_held<T, P, 128, 1>(a, vec, part, np, st);
       else if (a.cols <= 2048) s = norm_bwd_held<T, P, 256, 1>(a, vec, part, np, st);
-      else if (a.cols <= 4096) s = norm_bwd_held<T, P, 256, 2>(a, vec, part, np, st);
-      else if (a.cols <= 8192) s = norm_bwd_held<T, P, 512, 2>(a, vec, part, np, st);
+      else if (a.cols <= 4096) s = norm_bwd_held<T, P, 512, 1>(a, vec, part, np, st);
+      else if (a.cols <= 8192) s = norm_bwd_held<T, P, 1024, 1>(a, vec, part, np, st);
       else s = norm_bwd_held<T, P, 1024, 2>(a, vec, part, np, st);
     } else {
       if (a.g_x) {

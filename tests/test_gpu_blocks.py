@@ -581,3 +581,94 @@ def test_captured_and_replayed():
         for s, (graph, args, state, outs) in enumerate(made):
             for u, v in zip(outs, block_run(b, *args, (0.2, s, it))):
                 assert torch.equal(u, v), (it, s)
+
+
+# ---- sizes that take every tile, K split and fetch -------------------------------------------------------------------------------
+
+def check_on_gpu(got, want, tol, what):
+    d = (got.double() - want).abs()
+    bad = ~(d <= tol)
+    assert not bool(bad.any()), "%s: %d of %d off, worst |d| %.3e" % (what, int(bad.sum()), bad.numel(), float(d[bad].max()))
+
+
+BIG = [(4096, 520, 4104), (2048, 264, 4096), (2048, 1032, 2048), (1537, 1001, 777), (300, 4096, 512), (100, 8192, 264), (520, 130, 1000), (70, 2050, 4100),
+       (200, 6, 300), (90, 62, 130), (640, 126, 96), (130, 2, 70), (1000, 9, 65), (257, 4103, 129), (96, 640, 64), (97, 644, 68)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,inn,out", BIG)
+def test_linear_and_its_gradients_over_the_plans(rows, inn, out, dtype):
+    """The same definitions and tolerances as above, with the 64-bit products on the device."""
+    t = TYPES[dtype]
+    g = torch.Generator(device="cuda")
+    g.manual_seed(rows + inn + out)
+
+    def rnd(*shape, scale=1.0):
+        return (torch.randn(*shape, generator=g, device="cuda") * scale).to(t)
+
+    x, w, res = rnd(rows, inn), rnd(out, inn, scale=inn ** -0.5), rnd(rows, out)
+    eps, tiny = half(t)
+    xd, wd = x.double(), w.double()
+    z, mag = xd @ wd.t(), xd.abs() @ wd.abs().t()
+    want = torch.relu(z) + res.double()
+    dz = (inn + 1) * U * mag
+    check_on_gpu(blocks().linear(x, w, act="relu", residual=res), want, dz + (eps + U) * (want.abs() + dz) + tiny, "out")
+    go = rnd(rows, out)
+    gd = go.double()
+    g_x, g_w, g_b = blocks().linear_grad(go, x, w)
+    for got, want, mag, n, what in ((g_x, gd @ wd, gd.abs() @ wd.abs(), out, "g_x"), (g_w, gd.t() @ xd, gd.abs().t() @ xd.abs(), rows, "g_weight"),
+                                    (g_b, gd.sum(0), gd.abs().sum(0), rows, "g_bias")):
+        off = (n + 1) * U * mag
+        check_on_gpu(got, want, off + (eps + U) * (want.abs() + off) + tiny, what)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("inn,ld,start", [(131, 132, 0), (129, 134, 2), (65, 72, 4), (70, 74, 2), (33, 40, 8), (1, 2, 0), (7, 12, 4), (136, 140, 2)])
+def test_linear_rows_on_every_4_bytes(inn, ld, start, dtype):
+    """Rows that start at multiples of 4 bytes only, with a K that ends inside a 16-byte piece; what lies behind it is NaN."""
+    t = TYPES[dtype]
+    rng = np.random.RandomState(inn)
+    for rows, out in ((200, 130), (20, 24)):
+        x, w = (torch.full((n, ld + start), float("nan"), dtype=t, device="cuda")[:, start:start + inn] for n in (rows, out))
+        x.copy_(rand(rng, (rows, inn), t))
+        w.copy_(rand(rng, (out, inn), t, inn ** -0.5))
+        want, tol, _, _ = linear_want(x, w, None, "none", None, 0.0, t)
+        check(blocks().linear(x, w), want, tol, "out")
+        g = rand(rng, (rows, out), t)
+        wants, tols = linear_grad_want(g, x, w, None, "none", 0.0, t)
+        for got, a, b, what in zip(blocks().linear_grad(g, x, w), wants, tols, ("g_x", "g_weight", "g_bias")):
+            check(got, a, b, what)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_inputs_at_the_end_of_their_memory(dtype):
+    """The last row ends where its allocation ends, odd sizes: results as of a copy in the middle of a larger one."""
+    t = TYPES[dtype]
+    rng = np.random.RandomState(4)
+    for rows, inn, out in ((1, 4097, 33), (70, 259, 67), (300, 131, 257)):
+        total = rows * inn + 8
+        x = torch.empty(total, dtype=t, device="cuda")[total - rows * inn:].view(rows, inn)
+        x.copy_(rand(rng, (rows, inn), t))
+        w = rand(rng, (out, inn), t, 0.1)
+        roomy = torch.zeros(rows + 2, inn, dtype=t, device="cuda")
+        roomy[1:-1] = x
+        assert torch.equal(blocks().linear(x, w), blocks().linear(roomy[1:-1], w))
+        g = rand(rng, (rows, out), t)
+        for a, b in zip(blocks().linear_grad(g, x, w), blocks().linear_grad(g, roomy[1:-1], w)):
+            assert torch.equal(a, b)
+
+
+def test_linear_with_an_output_over_its_input_is_refused():
+    x = torch.zeros(64, 64, device="cuda")
+    w = torch.zeros(64, 64, device="cuda")
+    for out in (x, w):
+        with pytest.raises(ValueError, match="overlaps"):
+            blocks().linear(x, w, out=out)
+    wide = torch.zeros(64, 80, device="cuda")
+    with pytest.raises(ValueError, match="overlaps"):
+        blocks().linear(x, w, residual=wide[:, :64], out=wide[:, 8:72])
+    blocks().linear(x, w, residual=wide[:, :64], out=wide[:, :64])
+    blocks().linear(wide[:32, :64], w, out=wide[32:, :64])
+    both = torch.randn(64, 128, device="cuda")                   # columns side by side in one buffer
+    want = blocks().linear(both[:, :64].contiguous(), w)
+    assert torch.equal(blocks().linear(both[:, :64], w, out=both[:, 64:]), want)
