@@ -1,15 +1,15 @@
 // C[m, n] = epilogue(sum_k X(m, k) W(n, k)): the matrix product of the token blocks on the CDNA4 matrix pipe.
 //
 // A workgroup owns a BM x BN tile.  K is walked in steps of 128 bytes per row (64 elements of 16 bits, 32 of 32 bits); a step's
-// two operand tiles are moved by LDS-DMA (buffer_load_dwordx4 ... lds: 16 bytes per lane, no registers in between) into one of
-// two LDS stages while the other is multiplied.  Both memory orders of an operand are read as they lie:
+// two operand tiles are moved by LDS-DMA (buffer_load_dwordx4 ... lds: 16 bytes per lane, no registers in between) into a ring of 2
+// to 4 LDS stages while earlier ones are multiplied.  Both memory orders of an operand are read as they lie:
 //   K adjacent  LDS rows of 128 bytes, one per m (n); a lane's fragment is one ds_read_b128
 //   K strided   LDS rows of BM (BN) elements, one per k; fragments by the transposing ds_read_b64_tr_b16 (16 bit) or
 //               ds_read_b32 (32 bit)
 // with the 16-byte pieces of a row permuted by the row index (the lanes of the DMA fetch permuted addresses: LDS-DMA writes lane
 // after lane), so that the fragment reads of a wave spread over all banks.  Rows past M or N repeat the last one (not stored),
-// pieces past K are out of the buffer descriptor's range and arrive as zeros; the one that
-// K ends in comes through registers.
+// pieces past K are out of the buffer descriptor's range and arrive as zeros; the piece that
+// an adjacent K, or the last of strided k rows, ends in comes through registers.
 //
 // The product is taken as W X^T per wave (MFMA rows = n, columns = m): a lane then holds 4 adjacent n of one m.  Results pass
 // through LDS once more (32 rows of f32 per wave) so that every lane stores 8 adjacent columns, with bias, activation,
@@ -74,12 +74,6 @@ __device__ __forceinline__ void dma16(uint32_t lds, uint32_t voff, i32x4 srd) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(srd) : "memory");      // m0 is reserved: the compiler sets it before any use of its own
 #endif
 }
-// the same with 4 bytes per lane
-__device__ __forceinline__ void dma4(uint32_t lds, uint32_t voff, i32x4 srd) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(srd) : "memory");
-#endif
-}
 // everything this wave has in flight has landed, then all waves of the workgroup have got here
 __device__ __forceinline__ void barrier_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 // the same, with the N latest fetches of this wave still on their way
@@ -91,14 +85,13 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(
 
 constexpr uint32_t kOutside = 0x80000000u;      // = num_records: a lane with this offset reads zeros
 
-// One operand's tile of R rows (m or n) per K step: how it is fetched and how its fragments are read.  G: bytes that a lane fetches at
-// a time, 16, or 4 where the rows of a strided operand are not made of 16-byte pieces (then with four times the instructions).  The
-// addresses are multiples of 4.
-template <typename T, int R, bool S, int NT, int G, int MF>
+// One operand's tile of R rows (m or n) per K step: how it is fetched and how its fragments are read.  A lane fetches 16 bytes at a
+// time, from addresses that are multiples of 4.
+template <typename T, int R, bool S, int NT, int MF>
 struct Side {
-  static constexpr int E = sizeof(T), KS = 128 / E, PASSES = R * 128 / (NT * G);      // KS: k per step
+  static constexpr int E = sizeof(T), KS = 128 / E, PASSES = R * 128 / (NT * 16);      // KS: k per step
   static constexpr int ROWB = S ? R * E : 128;                                        // bytes of an LDS row
-  static_assert(R * 128 % (NT * G) == 0 && NT % 128 == 0 && (S || R % MF == 0) && (G == 16 || G == 4) && G >= E, "tile / threads");
+  static_assert(R * 128 % (NT * 16) == 0 && NT % 128 == 0 && (S || R % MF == 0), "tile / threads");
 
   // Where 16-byte piece `chunk` of row `row` lies in LDS, and back.  64 banks of 4 bytes serve 256 bytes a cycle; the lanes of one
   // cycle read  adjacent: 16 rows at one chunk | strided, 16 bit: 4 k rows x 2 neighbouring pairs of chunks | strided, 32 bit: 2 (4) k
@@ -121,8 +114,10 @@ struct Side {
   uint32_t voff[PASSES];    // buffer offset of this lane's piece in each pass
   int kpos;                 // and where along k the first one lies: adjacent, in bytes; strided, in rows
 
-  static constexpr int STEP = NT * G / ROWB;      // LDS rows from pass to pass
-  static_assert(NT * G % ROWB == 0, "a pass takes whole rows");
+  int cut;                  // strided: bit i: the piece of pass i is the one that the k rows end in
+
+  static constexpr int STEP = NT * 16 / ROWB;      // LDS rows from pass to pass
+  static_assert(NT * 16 % ROWB == 0, "a pass takes whole rows");
   // the same for pass i: the keys of rows STEP apart are the same, or differ in one bit
   __device__ __forceinline__ int kpos_of(int i) const {
     if constexpr (S) return kpos + i * STEP;
@@ -140,17 +135,22 @@ struct Side {
       step = (int64_t)KS * ld_;
       inner = (rows - r0) * E < R * E ? (int)(rows - r0) * E : R * E;
     }
-    const int at = threadIdx.x * G, row0 = at / ROWB, col = at % ROWB;
-    kpos = S ? row0 : chunk_of(col >> 4, row0) * 16 + (col & 15);
+    const int at = threadIdx.x * 16, row0 = at / ROWB, slot = at % ROWB >> 4;
+    kpos = S ? row0 : chunk_of(slot, row0) * 16;
+    cut = 0;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-      const int row = row0 + i * STEP, b = chunk_of(col >> 4, row) * 16 + (col & 15);
+      const int row = row0 + i * STEP, b = chunk_of(slot, row) * 16;
       if constexpr (!S) voff[i] = (uint32_t)(row < inner ? row : inner) * ld + b;
-      else voff[i] = b < inner ? row * ld + b : kOutside;
+      else {
+        voff[i] = b < inner ? row * ld + b : kOutside;
+        if (b < inner && b + 16 > inner) cut |= 1 << i;
+      }
     }
   }
   // the next step's tile: open, then one piece after the other into LDS at `lds`; left: what of K there is from the step's start on, in
-  // bytes (adjacent; a piece that is not whole is left out) or rows (strided), 0 or less: nothing
+  // bytes (adjacent) or rows (strided), 0 or less: nothing.  A piece that is not whole is left out; not so a strided one, whose
+  // other end lies in the next k row and falls to columns that are not stored -- but there is none after the last row.
   __device__ __forceinline__ void open() {
     const uint64_t b = (uint64_t)base;
     srd[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
@@ -160,9 +160,10 @@ struct Side {
     base += step;
   }
   __device__ __forceinline__ void piece(int i, uint32_t lds, int left) {
-    const uint32_t v = (S ? kpos_of(i) < left : kpos_of(i) + G <= left) ? voff[i] : kOutside;
-    if constexpr (G == 16) dma16(lds + i * NT * 16, v, srd);
-    else dma4(lds + i * NT * 4, v, srd);
+    bool in;
+    if constexpr (S) in = kpos_of(i) < left - (cut >> i & 1);
+    else in = kpos_of(i) + 16 <= left;
+    dma16(lds + i * NT * 16, in ? voff[i] : kOutside, srd);
   }
   // fragment of the MF rows from r on, k group kk, for Mma<T, MF>
   static __device__ __forceinline__ u32x4 frag(const char* tile, int r, int kk) {
@@ -195,12 +196,12 @@ struct Side {
   }
 };
 
-template <typename T, int MF, int TM, int TN, int WM, int WN, int NS, int G, bool XS, bool WS>
+template <typename T, int MF, int TM, int TN, int WM, int WN, int NS, bool XS, bool WS>
 __global__ __launch_bounds__(WM * WN * 64, 2) void token_tile_kernel(const TileArgs a) {
   constexpr int NT = WM * WN * 64, BM = WM * TM * MF, BN = WN * TN * MF, STAGE = (BM + BN) * 128;
   constexpr int PITCH = TN * MF + 4;
-  typedef Side<T, BM, XS, NT, G, MF> X;
-  typedef Side<T, BN, WS, NT, G, MF> W;
+  typedef Side<T, BM, XS, NT, MF> X;
+  typedef Side<T, BN, WS, NT, MF> W;
   typedef Mma<T, MF> I;
   extern __shared__ __attribute__((aligned(16))) char smem[];
 
@@ -218,7 +219,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void token_tile_kernel(const TileA
   W sw;
   sx.init(a.x, a.ld_x, m0, a.M, k0);
   sw.init(a.w, a.ld_w, n0, a.N, k0);
-  const uint32_t l0 = __builtin_amdgcn_readfirstlane(lds_addr(smem) + (threadIdx.x & ~63u) * G);      // this wave's lanes in each pass
+  const uint32_t l0 = __builtin_amdgcn_readfirstlane(lds_addr(smem) + (threadIdx.x & ~63u) * 16);      // this wave's lanes in each pass
   const int64_t k_end = (int64_t)k1 * X::KS < a.K ? (int64_t)k1 * X::KS : a.K;
   int64_t k_left = k_end - (int64_t)k0 * X::KS;
   // one of the PX + PW pieces of the next step's tiles
@@ -266,25 +267,44 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void token_tile_kernel(const TileA
   // not used (fetches out of range leave zeros).
   constexpr int P = PX + PW, NG = MF / 8, Q = NS == 2 ? P : (P + NG - 1) / NG;      // fetches in a group
   constexpr auto upto = [](int g) { return g * Q < P ? g * Q : P; };
-  // K adjacent and no multiple of 16 bytes: the last piece of each row, which the fetches leave out, comes element by element
-  // through registers, one row per lane; its elements past K are zeros
+  // What the fetches leave out comes element by element through registers, before the last step's fragments are read.  K adjacent: the
+  // piece that each row ends in, a row per lane, zeros past K.  K strided: the piece that the last k row of the range ends in.
   static_assert(NT >= BM + BN, "a row per lane");
   constexpr int V = 16 / (int)sizeof(T);
   const int row = threadIdx.x, odd = (int)(a.K % V);
-  const bool ragged = odd != 0 && k1 == a.nk && !(XS && WS);
+  const bool ends = !(XS && WS) && odd != 0 && k1 == a.nk;
+  const bool cut_x = XS && a.M - m0 < BM && (a.M - m0) % V != 0, cut_w = WS && a.N - n0 < BN && (a.N - n0) % V != 0;
+  const bool ragged = ends || cut_x || cut_w;
   u32x4 tail = {0, 0, 0, 0};
   char* tail_to = nullptr;
-  if (ragged && (row < BM ? !XS : row < BM + BN && !WS)) {
-    const int r = row < BM ? row : row - BM;
-    const int64_t at = row < BM ? (m0 + r < a.M ? m0 + r : a.M - 1) * a.ld_x : (n0 + r < a.N ? n0 + r : a.N - 1) * a.ld_w;
-    const T* from = (const T*)((row < BM ? a.x : a.w) + at) + (a.K - odd);
-    T v[V];
+  if (ragged) {
+    const T* from = nullptr;
+    int count = 0;
+    const bool in_x = row < BM;
+    const int r = in_x ? row : row - BM;
+    if (in_x ? XS : WS) {
+      if (r == 0 && (in_x ? cut_x : cut_w)) {
+        const int64_t left = in_x ? a.M - m0 : a.N - n0, first = left / V * V;
+        count = (int)(left - first);
+        from = (const T*)((in_x ? a.x : a.w) + (k_end - 1) * (in_x ? a.ld_x : a.ld_w)) + (in_x ? m0 : n0) + first;
+        const int krow = (int)((k_end - 1) % X::KS), chunk = (int)(first / V);
+        if constexpr (XS) { if (in_x) tail_to = smem + krow * X::ROWB + (X::slot_of(chunk, krow) << 4); }
+        if constexpr (WS) { if (!in_x) tail_to = smem + BM * 128 + krow * W::ROWB + (W::slot_of(chunk, krow) << 4); }
+      }
+    } else if (ends && row < BM + BN) {
+      count = odd;
+      const int64_t at = in_x ? (m0 + r < a.M ? m0 + r : a.M - 1) * a.ld_x : (n0 + r < a.N ? n0 + r : a.N - 1) * a.ld_w;
+      from = (const T*)((in_x ? a.x : a.w) + at) + (a.K - odd);
+      const int chunk = (int)((a.K - odd) * (int64_t)sizeof(T) % 128) >> 4;
+      if constexpr (!XS) { if (in_x) tail_to = smem + r * 128 + (X::slot_of(chunk, r) << 4); }
+      if constexpr (!WS) { if (!in_x) tail_to = smem + BM * 128 + r * 128 + (W::slot_of(chunk, r) << 4); }
+    }
+    if (count > 0) {
+      T v[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = j < odd ? from[j] : (T)0.f;
-    __builtin_memcpy(&tail, v, 16);
-    const int chunk = (int)((a.K - odd) * (int64_t)sizeof(T) % 128) >> 4;
-    if constexpr (!XS) { if (row < BM) tail_to = smem + r * 128 + (X::slot_of(chunk, r) << 4); }
-    if constexpr (!WS) { if (row >= BM) tail_to = smem + BM * 128 + r * 128 + (W::slot_of(chunk, r) << 4); }
+      for (int j = 0; j < V; ++j) v[j] = j < count ? from[j] : (T)0.f;
+      __builtin_memcpy(&tail, v, 16);
+    }
   }
   auto add_tail = [&](int stage) {
     if (tail_to) *(u32x4*)(tail_to + stage * STAGE) = tail;
@@ -400,19 +420,24 @@ struct FewArgs {
   Epilogue e;
 };
 
-// 16 bytes of a row at byte b; zeros past its end.  VEC: rows are whole 16-byte pieces, aligned
+// 16 bytes of a row at byte b; zeros past its end.  VEC: rows are whole 16-byte pieces, aligned; else a load of any alignment (which
+// the hardware takes, a little slower), and the row's last piece element by element
 template <typename T, bool VEC>
 __device__ __forceinline__ u32x4 row_piece(const char* row, int b, int kb) {
+  typedef u32x4 __attribute__((aligned(2))) any16;
   u32x4 v = {0, 0, 0, 0};
   if constexpr (VEC) {
     if (b < kb) v = *(const u32x4*)(row + b);
-  } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) if (b + 4 * j < kb) v[j] = *(const uint32_t*)(row + b + 4 * j);
+  } else if (b + 16 <= kb) {
+    v = *(const any16*)(row + b);
   } else {
+    constexpr int E = sizeof(T);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (b + 2 * j < kb) v[j >> 1] |= (uint32_t)*(const uint16_t*)(row + b + 2 * j) << (16 * (j & 1));
+    for (int j = 0; j < 16 / E; ++j)
+      if (b + E * j < kb) {
+        if constexpr (E == 4) v[j] = *(const uint32_t*)(row + b + 4 * j);
+        else v[j >> 1] |= (uint32_t)*(const uint16_t*)(row + b + 2 * j) << (16 * (j & 1));
+      }
   }
   return v;
 }
@@ -438,7 +463,7 @@ __global__ __launch_bounds__(512, 1) void token_few_kernel(const FewArgs a) {
   f32x4 acc[MB];
 #pragma unroll
   for (int i = 0; i < MB; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  constexpr int U = VEC ? (MB == 1 ? 4 : 2) : 1;      // pieces in flight
+  constexpr int U = MB == 1 ? 4 : MB == 2 || VEC ? 2 : 1;      // pieces in flight
   for (int b0 = wave * 128; b0 < a.kb; b0 += 1024 * U) {
     u32x4 fw[U][2], fx[U][2][MB];
 #pragma unroll
@@ -516,7 +541,7 @@ __global__ __launch_bounds__(256) void token_join_kernel(const float* __restrict
   }
 }
 
-// dst [rows][cols_pad] = src [rows][cols], zeros behind: an operand whose rows are not 16-byte pieces
+// dst [rows][cols_pad] = src [rows][cols], zeros behind: an operand that the tiles cannot fetch as it lies
 template <typename U>
 __global__ __launch_bounds__(256) void token_pack_kernel(const U* __restrict__ src, int64_t ld, U* __restrict__ dst, int64_t rows, int cols, int cols_pad) {
   constexpr int V = 16 / sizeof(U);
@@ -539,20 +564,17 @@ struct Plan {
   int few;                   // 16-row blocks of token_few_kernel, 0: tiles
   int tile;                  // index into the tile table
   int nsplit;
-  int fetch;                 // bytes per lane
   bool pack_x, pack_w;
   int64_t ldp_x, ldp_w;      // elements, packed
   int64_t x_off, w_off, part_off, bytes, ld_part;
 };
 
-// bytes that a lane can fetch at a time, 0: the operand has to be copied first.  Pieces of 16 need rows that start at multiples of 4
-// bytes, and for a strided operand rows of whole pieces (what is past K is made up by the kernel, what is past M or N would
-// be past the operand's end).  A tile's rows have to lie within the 2 GiB that an offset of the buffer descriptor spans.
-int fetch_bytes(const Operand& o, int64_t rows, int E) {
-  if ((o.strided ? 128 / E : 256) * o.ld * E >= (1ll << 31) - 65536) return 0;
-  if (((uint64_t)(uintptr_t)o.p | (uint64_t)(o.ld * E)) & 3) return 0;
-  if (!o.strided || o.padded || (rows * E) % 16 == 0) return 16;
-  return (rows * E) % 4 == 0 ? 4 : 0;
+// whether an operand has to be copied first: its rows do not all start at multiples of 4 bytes, or a tile's rows span more than the 2 GiB
+// that an offset of the buffer descriptor does, or the k rows lie so close that the 16 bytes a row ends in may reach past the last one
+bool needs_pack(const Operand& o, int64_t rows, int E) {
+  if ((o.strided ? 128 / E : 256) * o.ld * E >= (1ll << 31) - 65536) return true;
+  if (o.strided && o.ld * E < 16 && rows * E % 16) return true;
+  return (((uint64_t)(uintptr_t)o.p | (uint64_t)(o.ld * E)) & 3) != 0;
 }
 
 // The tiles and what they cost, measured over 20 shapes from 32 x 4096 x 4096 to 8192 x 16384 x 4096 (128 to 8192 workgroups, K splits 1
@@ -571,21 +593,20 @@ Plan make_plan(const Product& p) {
   const int E = (int)dtype_bytes(p.dtype), V = 16 / E;
   Plan o = {};
   // token_few_kernel reads X again for every 16 columns, the tiles in whole tile rows: at 16 rows and 4096 x 4096 weights (bf16) 11.0 us
-  // against 14.7, at 32 rows 13.9 against 12.7; up to 64 rows where there is little to read at all (1024 x 1024: 7.0 against 8.3)
-  if (!p.x.strided && !p.w.strided && (p.M <= 16 || (p.M <= 64 && p.M * p.N * p.K <= 1 << 26))) {
+  // against 14.7, at 32 rows 13.9 against 12.7; up to 64 rows where there is little to read at all (1024 x 1024: 7.0 against 8.3) and
+  // rows are short (48 rows, 160 x 7376, odd rows: 66 us, as its 10 workgroups go along K alone; the tiles, which split K, 16)
+  if (!p.x.strided && !p.w.strided && (p.M <= 16 || (p.M <= 64 && p.K * E <= 4096 && p.M * p.N * p.K <= 1 << 26))) {
     o.few = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
     return o;
   }
-  const int gx = fetch_bytes(p.x, p.M, E), gw = fetch_bytes(p.w, p.N, E);
-  o.pack_x = gx == 0;
-  o.pack_w = gw == 0;
-  o.fetch = gx == 4 || gw == 4 ? 4 : 16;
+  o.pack_x = needs_pack(p.x, p.M, E);
+  o.pack_w = needs_pack(p.w, p.N, E);
   if (o.pack_x) { o.ldp_x = round_up(p.x.strided ? p.M : p.K, V); o.x_off = o.bytes; o.bytes += round_up((p.x.strided ? p.K : p.M) * o.ldp_x * E, 256); }
   if (o.pack_w) { o.ldp_w = round_up(p.w.strided ? p.N : p.K, V); o.w_off = o.bytes; o.bytes += round_up((p.w.strided ? p.K : p.N) * o.ldp_w * E, 256); }
   const int64_t nk = ceil_div(p.K, 128 / E);
   // rows off the 16-byte grid cost a lone workgroup a fifth more per step (two on a CU cover it for each other); results that leave
   // element by element, 4 us more at the end of a tile, which the join's many small workgroups do not feel
-  const bool off = o.fetch == 4 || (((uint64_t)(uintptr_t)p.x.p | (uint64_t)(p.x.ld * E) | (uint64_t)(uintptr_t)p.w.p | (uint64_t)(p.w.ld * E)) & 15);
+  const bool off = (((uint64_t)(uintptr_t)p.x.p | (uint64_t)(p.x.ld * E) | (uint64_t)(uintptr_t)p.w.p | (uint64_t)(p.w.ld * E)) & 15) != 0;
   double best = 1e300;
   o.nsplit = 1;
   for (int t = 0; t < kTiles; ++t) {
@@ -607,33 +628,33 @@ Plan make_plan(const Product& p) {
   return o;
 }
 
-template <typename T, int MF, int TM, int TN, int WM, int WN, int NS, int G, bool XS, bool WS>
+template <typename T, int MF, int TM, int TN, int WM, int WN, int NS, bool XS, bool WS>
 int run_tile(const TileArgs& a, hipStream_t st) {
   constexpr int BM = WM * TM * MF, BN = WN * TN * MF, MAIN = NS * (BM + BN) * 128, EPI = WM * WN * MF * (TN * MF + 4) * 4;
   constexpr int LDS = MAIN > EPI ? MAIN : EPI;
-  const void* f = reinterpret_cast<const void*>(&token_tile_kernel<T, MF, TM, TN, WM, WN, NS, G, XS, WS>);
+  const void* f = reinterpret_cast<const void*>(&token_tile_kernel<T, MF, TM, TN, WM, WN, NS, XS, WS>);
   if (LDS > 65536 && hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return SGA_ERR_HIP;
-  hipLaunchKernelGGL((token_tile_kernel<T, MF, TM, TN, WM, WN, NS, G, XS, WS>), dim3((unsigned)(a.ntm * a.ntn * a.nsplit)), dim3(WM * WN * 64), LDS, st, a);
+  hipLaunchKernelGGL((token_tile_kernel<T, MF, TM, TN, WM, WN, NS, XS, WS>), dim3((unsigned)(a.ntm * a.ntn * a.nsplit)), dim3(WM * WN * 64), LDS, st, a);
   LAUNCHED();
   return SGA_OK;
 }
-template <typename T, int G, bool XS, bool WS>
+template <typename T, bool XS, bool WS>
 int run_tile_of(int tile, const TileArgs& a, hipStream_t st) {
   switch (tile) {
-    case 0: return run_tile<T, 32, 2, 4, 4, 2, 2, G, XS, WS>(a, st);
-    case 1: return run_tile<T, 32, 2, 2, 4, 2, 3, G, XS, WS>(a, st);
-    case 2: return run_tile<T, 32, 1, 2, 4, 2, 4, G, XS, WS>(a, st);
+    case 0: return run_tile<T, 32, 2, 4, 4, 2, 2, XS, WS>(a, st);
+    case 1: return run_tile<T, 32, 2, 2, 4, 2, 3, XS, WS>(a, st);
+    case 2: return run_tile<T, 32, 1, 2, 4, 2, 4, XS, WS>(a, st);
     case 3:
-      if constexpr (!XS) return run_tile<T, 16, 3, 2, 2, 2, 4, G, XS, WS>(a, st);
+      if constexpr (!XS) return run_tile<T, 16, 3, 2, 2, 2, 4, XS, WS>(a, st);
       return SGA_ERR_UNSUPPORTED;      // 96 rows of a strided X: make_plan takes another tile
-    default: return run_tile<T, 32, 1, 1, 2, 2, 4, G, XS, WS>(a, st);
+    default: return run_tile<T, 32, 1, 1, 2, 2, 4, XS, WS>(a, st);
   }
 }
-template <typename T, int G>
+template <typename T>
 int run_order(int tile, bool xs, bool ws, const TileArgs& a, hipStream_t st) {
-  if constexpr (G == 16) { if (!xs && !ws) return run_tile_of<T, G, false, false>(tile, a, st); }
-  if (!xs) return run_tile_of<T, G, false, true>(tile, a, st);
-  return run_tile_of<T, G, true, true>(tile, a, st);
+  if (!xs && !ws) return run_tile_of<T, false, false>(tile, a, st);
+  if (!xs) return run_tile_of<T, false, true>(tile, a, st);
+  return run_tile_of<T, true, true>(tile, a, st);
 }
 
 template <typename T, int MB>
@@ -679,7 +700,7 @@ int run(const Product& p, char* ws, hipStream_t st) {
   a.ld_part = o.ld_part;
   a.e = p.e;
   if ((int64_t)a.ntm * a.ntn * a.nsplit > 0x7fffffff) return SGA_ERR_UNSUPPORTED;
-  s = o.fetch == 16 ? run_order<T, 16>(o.tile, p.x.strided, p.w.strided, a, st) : run_order<T, 4>(o.tile, p.x.strided, p.w.strided, a, st);
+  s = run_order<T>(o.tile, p.x.strided, p.w.strided, a, st);
   if (s != SGA_OK || o.nsplit == 1) return s;
   if (p.e.vec)
     hipLaunchKernelGGL((token_join_kernel<T, true>), dim3((unsigned)ceil_div(p.M * (o.ld_part / 8), 256)), dim3(256), 0, st, a.part, o.nsplit, p.M, o.ld_part, p.e);
