@@ -291,8 +291,7 @@ __device__ __forceinline__ void epilogue1(const Epilogue& e, uint64_t seed, uint
 
 // ---- C[m, n] = epilogue(sum_k X(m, k) W(n, k)) (token_product.hip) -------------------------------------------------------
 // strided = 0: operand(r, k) = p[r ld + k]; strided = 1: operand(r, k) = p[k ld + r]
-// padded: rows (as they lie) are followed by zeros up to the next 16 bytes
-struct Operand { const void* p; int64_t ld; int strided; int padded; };
+struct Operand { const void* p; int64_t ld; int strided; };
 struct Product {
   Operand x, w;
   int64_t M, N, K;

@@ -196,6 +196,14 @@ struct Side {
   }
 };
 
+// Bound by the matrix pipe where K and the tiles are many.  8192 x 16384 x 4096 bf16, gelu, pre: 988 us = 1110 TFLOP/s, where a library
+// product alone takes 833; both run into the power limit there (on zeros this one reaches 1430).  Tiles by cost (kTile below): 2 x 4
+// results of 32 x 32 a wave read 6 fragments for 8 products, 1 x 2 read 3 for 2.  128 bytes of K a step: 64-byte steps in a deeper ring
+// were slower throughout, a 256 x 256 tile as 4 waves of 4 x 4 too.  Two waves per
+// SIMD are asked for so that the sums stay in ordinary registers: as accumulation registers they cost a move each at the end.
+// 8192 x 2048 x 8192 (bf16) with X adjacent and W strided: 225 us, both strided: 229 (1220, 1200 TFLOP/s; library 208).
+// 2048 x 2048 x 8192 with residual and dropout: 79 us = 875 TFLOP/s, 256 workgroups of 128 x 128, one each: its start and end lie
+// bare.  f32 1537 x 777 x 1001: 34 us + join 6, one wave of tiles with the pipe at half its rate.
 template <typename T, int MF, int TM, int TN, int WM, int WN, int NS, bool XS, bool WS>
 __global__ __launch_bounds__(WM * WN * 64, 2) void token_tile_kernel(const TileArgs a) {
   constexpr int NT = WM * WN * 64, BM = WM * TM * MF, BN = WN * TN * MF, STAGE = (BM + BN) * 128;
@@ -412,6 +420,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void token_tile_kernel(const TileA
 // A workgroup of 8 waves owns 16 columns n.  The waves share out K in pieces of 128 bytes per row of w, so that a wave reads whole
 // lines; MFMA rows = the 16 columns, MFMA columns = 16 rows of X (MB of them).  Any order of k inside a piece serves, as both
 // operands take the same: lane (r, q) takes bytes q * 16 .. of each 64.  The waves' sums meet in LDS.
+// Bound by the weight's bytes and, when small, by latency: one row of 4096 x 4096 bf16 (34 MB) 7.9 us = 4.2 TB/s, 12 rows of
+// 10240 x 2560 f16 (52 MB) 15 us = 3.5 TB/s.  Up to 4 pieces in flight a wave, as the registers allow.
 struct FewArgs {
   const char* x; const char* w;
   int64_t ld_x, ld_w;            // bytes
@@ -420,29 +430,40 @@ struct FewArgs {
   Epilogue e;
 };
 
-// 16 bytes of a row at byte b; zeros past its end.  VEC: rows are whole 16-byte pieces, aligned; else a load of any alignment (which
-// the hardware takes, a little slower), and the row's last piece element by element
-template <typename T, bool VEC>
-__device__ __forceinline__ u32x4 row_piece(const char* row, int b, int kb) {
-  typedef u32x4 __attribute__((aligned(2))) any16;
-  u32x4 v = {0, 0, 0, 0};
-  if constexpr (VEC) {
-    if (b < kb) v = *(const u32x4*)(row + b);
-  } else if (b + 16 <= kb) {
-    v = *(const any16*)(row + b);
-  } else {
-    constexpr int E = sizeof(T);
+// How rows lie: every 16-byte piece aligned and whole | starts at multiples of 4 bytes | at any element (16-bit types).  Pieces
+// that start inside a word are put together from the five words that hold them: one row of 4096 x 4096, stride 4097, 13.9 us, against 17.1
+// with loads that straddle words (8.3 for stride 4098, 7.9 for 4096).
+enum { kPieces, kWords, kElements };
+// a whole piece
+template <int ROWS>
+__device__ __forceinline__ u32x4 row_piece(const char* p) {
+  typedef u32x4 __attribute__((aligned(4))) words;
+  if constexpr (ROWS == kPieces) return *(const u32x4*)p;
+  if constexpr (ROWS == kWords) return *(const words*)p;
+  const uint32_t odd = (uint32_t)(uintptr_t)p & 2;
+  p -= odd;
+  u32x4 v = *(const words*)p;
+  const uint32_t last = *(const uint32_t*)(p + (odd ? 16 : 12));      // no word that holds nothing of the row is touched
 #pragma unroll
-    for (int j = 0; j < 16 / E; ++j)
-      if (b + E * j < kb) {
-        if constexpr (E == 4) v[j] = *(const uint32_t*)(row + b + 4 * j);
-        else v[j >> 1] |= (uint32_t)*(const uint16_t*)(row + b + 2 * j) << (16 * (j & 1));
-      }
+  for (int j = 0; j < 3; ++j) v[j] = __builtin_amdgcn_alignbyte(v[j + 1], v[j], odd);
+  v[3] = __builtin_amdgcn_alignbyte(last, v[3], odd);
+  return v;
+}
+// the piece that a row ends in: n bytes, zeros behind.  No branches: the loads leave together.
+template <typename T>
+__device__ __forceinline__ u32x4 row_end(const char* p, int n) {
+  constexpr int E = sizeof(T);
+  typedef typename std::conditional<E == 4, uint32_t, uint16_t>::type U;
+  u32x4 v = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 16 / E; ++j) {
+    const uint32_t u = *(const U*)(p + (E * j < n ? E * j : 0));
+    v[j * E / 4] |= E * j < n ? u << (E * j % 4 * 8) : 0u;
   }
   return v;
 }
 
-template <typename T, int MB, bool VEC>
+template <typename T, int MB, int ROWS>
 __global__ __launch_bounds__(512, 1) void token_few_kernel(const FewArgs a) {
   __shared__ __attribute__((aligned(16))) float sh[8][MB * 16][20];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
@@ -463,17 +484,33 @@ __global__ __launch_bounds__(512, 1) void token_few_kernel(const FewArgs a) {
   f32x4 acc[MB];
 #pragma unroll
   for (int i = 0; i < MB; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  constexpr int U = MB == 1 ? 4 : MB == 2 || VEC ? 2 : 1;      // pieces in flight
-  for (int b0 = wave * 128; b0 < a.kb; b0 += 1024 * U) {
+  constexpr int U = MB == 1 ? 4 : MB == 2 || ROWS != kElements ? 2 : 1;      // pieces in flight
+  const int whole = ROWS == kPieces ? a.kb : a.kb & ~15;
+  // where rows end inside a piece, the last wave, which has the least to do, takes it by itself
+  const bool ends = ROWS != kPieces && wave == 7 && whole < a.kb;
+  u32x4 ew = {0, 0, 0, 0}, ex[MB] = {};
+  if constexpr (ROWS != kPieces) {
+    if (ends && q == 0) {
+      ew = row_end<T>(wrow + whole, a.kb - whole);
+#pragma unroll
+      for (int i = 0; i < MB; ++i) ex[i] = row_end<T>(xrow[i] + whole, a.kb - whole);
+    }
+  }
+  for (int b0 = wave * 128; b0 < whole; b0 += 1024 * U) {
     u32x4 fw[U][2], fx[U][2][MB];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int b = b0 + u * 1024 + h * 64 + q * 16;
-        fw[u][h] = row_piece<T, VEC>(wrow, b, a.kb);
+        fw[u][h] = u32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < MB; ++i) fx[u][h][i] = row_piece<T, VEC>(xrow[i], b, a.kb);
+        for (int i = 0; i < MB; ++i) fx[u][h][i] = u32x4{0, 0, 0, 0};
+        if (b < whole) {
+          fw[u][h] = row_piece<ROWS>(wrow + b);
+#pragma unroll
+          for (int i = 0; i < MB; ++i) fx[u][h][i] = row_piece<ROWS>(xrow[i] + b);
+        }
       }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -483,6 +520,14 @@ __global__ __launch_bounds__(512, 1) void token_few_kernel(const FewArgs a) {
         for (int j = 0; j < (sizeof(T) == 4 ? 4 : 1); ++j)
 #pragma unroll
           for (int i = 0; i < MB; ++i) acc[i] = Mma<T, 16>::mma1(fw[u][h], fx[u][h][i], j, acc[i]);
+  }
+  if constexpr (ROWS != kPieces) {
+    if (ends) {
+#pragma unroll
+      for (int j = 0; j < (sizeof(T) == 4 ? 4 : 1); ++j)
+#pragma unroll
+        for (int i = 0; i < MB; ++i) acc[i] = Mma<T, 16>::mma1(ew, ex[i], j, acc[i]);
+    }
   }
 #pragma unroll
   for (int i = 0; i < MB; ++i) *(f32x4*)&sh[wave][i * 16 + r][q * 4] = acc[i];
@@ -513,7 +558,8 @@ __global__ __launch_bounds__(512, 1) void token_few_kernel(const FewArgs a) {
   }
 }
 
-// out = epilogue(sum of the slabs, in their order): 8 columns per lane, or one where the rows' pieces are not whole
+// out = epilogue(sum of the slabs, in their order): 8 columns per lane, or one where the rows' pieces are not whole.  Bound by the
+// slabs' way in from L2: 2 of 1537 x 777 with residual (15 MB) 5.5 us.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void token_join_kernel(const float* __restrict__ part, int nsplit, int64_t M, int64_t ld_part, const Epilogue e) {
   uint64_t seed = 0, offset = 0;
@@ -541,7 +587,8 @@ __global__ __launch_bounds__(256) void token_join_kernel(const float* __restrict
   }
 }
 
-// dst [rows][cols_pad] = src [rows][cols], zeros behind: an operand that the tiles cannot fetch as it lies
+// dst [rows][cols_pad] = src [rows][cols], zeros behind: an operand that the tiles cannot fetch as it lies.
+// Bound by latency at the sizes it is met at: 160 x 7376 bf16, odd rows, 2.9 us
 template <typename U>
 __global__ __launch_bounds__(256) void token_pack_kernel(const U* __restrict__ src, int64_t ld, U* __restrict__ dst, int64_t rows, int cols, int cols_pad) {
   constexpr int V = 16 / sizeof(U);
@@ -661,10 +708,11 @@ template <typename T, int MB>
 int run_few(const Product& p, hipStream_t st) {
   const int64_t E = sizeof(T);
   const FewArgs a = {(const char*)p.x.p, (const char*)p.w.p, p.x.ld * E, p.w.ld * E, p.M, p.N, (int)(p.K * E), p.e};
-  const bool vec = !(((uintptr_t)a.x | (uintptr_t)a.w | (uint64_t)a.ld_x | (uint64_t)a.ld_w | (uint64_t)a.kb) & 15);
+  const uint64_t rows = (uintptr_t)a.x | (uintptr_t)a.w | (uint64_t)a.ld_x | (uint64_t)a.ld_w;
   const dim3 grid((unsigned)ceil_div(p.N, 16));
-  if (vec) hipLaunchKernelGGL((token_few_kernel<T, MB, true>), grid, dim3(512), 0, st, a);
-  else hipLaunchKernelGGL((token_few_kernel<T, MB, false>), grid, dim3(512), 0, st, a);
+  if (!((rows | (uint64_t)a.kb) & 15)) hipLaunchKernelGGL((token_few_kernel<T, MB, kPieces>), grid, dim3(512), 0, st, a);
+  else if (sizeof(T) == 4 || !(rows & 3)) hipLaunchKernelGGL((token_few_kernel<T, MB, kWords>), grid, dim3(512), 0, st, a);
+  else if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((token_few_kernel<T, MB, kElements>), grid, dim3(512), 0, st, a);
   LAUNCHED();
   return SGA_OK;
 }
