@@ -417,11 +417,13 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void token_tile_kernel(const TileA
 }
 
 // ---- few rows of X (tokens of as many sequences): the weight's rows are read once, straight into fragments ------------------
-// A workgroup of 8 waves owns 16 columns n.  The waves share out K in pieces of 128 bytes per row of w, so that a wave reads whole
+// A workgroup of 8 waves owns 16 columns n, or 8 where 16 would leave CUs idle (1 x 8192 x 2048 bf16: 9.3 us, with 16 columns 12.0; 16 rows 14.5
+// against 16.9).  The waves share out K in pieces of 128 bytes per row of w, so that a wave reads whole
 // lines; MFMA rows = the 16 columns, MFMA columns = 16 rows of X (MB of them).  Any order of k inside a piece serves, as both
 // operands take the same: lane (r, q) takes bytes q * 16 .. of each 64.  The waves' sums meet in LDS.
-// Bound by the weight's bytes and, when small, by latency: one row of 4096 x 4096 bf16 (34 MB) 7.9 us = 4.2 TB/s, 12 rows of
-// 10240 x 2560 f16 (52 MB) 15 us = 3.5 TB/s.  Up to 4 pieces in flight a wave, as the registers allow.
+// Bound by the weight's bytes and, when small, by latency: one row of 4096 x 4096 bf16 (34 MB) 8.2 us = 4.1 TB/s, 12 rows of
+// 10240 x 2560 f16 (52 MB) 15 us = 3.5 TB/s.  Up to 4 pieces in flight a wave, as the registers
+// allow (2 or 6: 8.9 us), through the caches (past them: 9.0, 12 rows 20.6).
 struct FewArgs {
   const char* x; const char* w;
   int64_t ld_x, ld_w;            // bytes
@@ -463,11 +465,11 @@ __device__ __forceinline__ u32x4 row_end(const char* p, int n) {
   return v;
 }
 
-template <typename T, int MB, int ROWS>
+template <typename T, int MB, int ROWS, int COLS>
 __global__ __launch_bounds__(512, 1) void token_few_kernel(const FewArgs a) {
   __shared__ __attribute__((aligned(16))) float sh[8][MB * 16][20];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int64_t n0 = (int64_t)blockIdx.x * COLS;
   const char* xrow[MB];
   const char* wrow = a.w + (n0 + r < a.N ? n0 + r : a.N - 1) * a.ld_w;
 #pragma unroll
@@ -477,7 +479,7 @@ __global__ __launch_bounds__(512, 1) void token_few_kernel(const FewArgs a) {
   const int64_t no = n0 + (threadIdx.x & 1) * 8;
   float b8[8] = {};
   Raw8<T> res = {};
-  if (a.e.vec && mo < a.M && no < a.N) {
+  if (a.e.vec && mo < a.M && (threadIdx.x & 1) * 8 < COLS && no < a.N) {
     bias8<T>(a.e, no, b8);
     res = residual8<T>(a.e, mo, no);
   }
@@ -507,7 +509,7 @@ __global__ __launch_bounds__(512, 1) void token_few_kernel(const FewArgs a) {
 #pragma unroll
         for (int i = 0; i < MB; ++i) fx[u][h][i] = u32x4{0, 0, 0, 0};
         if (b < whole) {
-          fw[u][h] = row_piece<ROWS>(wrow + b);
+          if (r < COLS) fw[u][h] = row_piece<ROWS>(wrow + b);      // 8 columns: the other lanes fetch nothing
 #pragma unroll
           for (int i = 0; i < MB; ++i) fx[u][h][i] = row_piece<ROWS>(xrow[i] + b);
         }
@@ -536,7 +538,7 @@ __global__ __launch_bounds__(512, 1) void token_few_kernel(const FewArgs a) {
   if (a.e.drop.on) drop_key(a.e.drop, seed, offset);
   if (a.e.vec) {
     const int m = threadIdx.x >> 1, c = (threadIdx.x & 1) * 8;
-    if (m >= a.M || n0 + c >= a.N) return;
+    if (m >= a.M || c >= COLS || n0 + c >= a.N) return;
     float v[8], u[8];
     load8(&sh[0][m][c], v);
 #pragma unroll
@@ -549,7 +551,7 @@ __global__ __launch_bounds__(512, 1) void token_few_kernel(const FewArgs a) {
   } else {
     for (int i = threadIdx.x; i < MB * 256; i += 512) {
       const int64_t m = i >> 4, n = n0 + (i & 15);
-      if (m >= a.M || n >= a.N) continue;
+      if (m >= a.M || (i & 15) >= COLS || n >= a.N) continue;
       float v = sh[0][m][i & 15];
 #pragma unroll
       for (int s = 1; s < 8; ++s) v += sh[s][m][i & 15];
@@ -709,10 +711,15 @@ int run_few(const Product& p, hipStream_t st) {
   const int64_t E = sizeof(T);
   const FewArgs a = {(const char*)p.x.p, (const char*)p.w.p, p.x.ld * E, p.w.ld * E, p.M, p.N, (int)(p.K * E), p.e};
   const uint64_t rows = (uintptr_t)a.x | (uintptr_t)a.w | (uint64_t)a.ld_x | (uint64_t)a.ld_w;
-  const dim3 grid((unsigned)ceil_div(p.N, 16));
-  if (!((rows | (uint64_t)a.kb) & 15)) hipLaunchKernelGGL((token_few_kernel<T, MB, kPieces>), grid, dim3(512), 0, st, a);
-  else if (sizeof(T) == 4 || !(rows & 3)) hipLaunchKernelGGL((token_few_kernel<T, MB, kWords>), grid, dim3(512), 0, st, a);
-  else if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((token_few_kernel<T, MB, kElements>), grid, dim3(512), 0, st, a);
+  auto launch = [&](auto columns) {
+    constexpr int COLS = decltype(columns)::value;
+    const dim3 grid((unsigned)ceil_div(p.N, COLS));
+    if (!((rows | (uint64_t)a.kb) & 15)) hipLaunchKernelGGL((token_few_kernel<T, MB, kPieces, COLS>), grid, dim3(512), 0, st, a);
+    else if (sizeof(T) == 4 || !(rows & 3)) hipLaunchKernelGGL((token_few_kernel<T, MB, kWords, COLS>), grid, dim3(512), 0, st, a);
+    else if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((token_few_kernel<T, MB, kElements, COLS>), grid, dim3(512), 0, st, a);
+  };
+  if (p.N <= 8 * kCUs) launch(std::integral_constant<int, 8>());
+  else launch(std::integral_constant<int, 16>());
   LAUNCHED();
   return SGA_OK;
 }

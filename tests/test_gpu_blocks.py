@@ -658,6 +658,21 @@ def test_inputs_at_the_end_of_their_memory(dtype):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("out", [3, 8, 12, 24, 2047, 2048, 2049, 2056])
+@pytest.mark.parametrize("rows,inn,gap", [(1, 200, 0), (16, 1031, 0), (13, 75, 1), (33, 300, 2), (50, 129, 1), (2, 7, 1), (5, 8, 1)])
+def test_linear_of_few_rows(rows, inn, gap, out, dtype):
+    """Few rows on every alignment, rows that end inside a piece, and column blocks of 8 and 16 whose last one is short; NaN in the gaps."""
+    t = TYPES[dtype]
+    rng = np.random.RandomState(rows + inn + out)
+    x, w = (torch.full((n, inn + gap), float("nan"), dtype=t, device="cuda")[:, :inn] for n in (rows, out))
+    x.copy_(rand(rng, (rows, inn), t))
+    w.copy_(rand(rng, (out, inn), t, inn ** -0.5))
+    bias, res = rand(rng, (out,), t), rand(rng, (rows, out), t)
+    want, tol, _, _ = linear_want(x, w, bias, "none", res, 0.0, t)
+    check(blocks().linear(x, w, bias, residual=res), want, tol, "out")
+
+
 def test_linear_with_an_output_over_its_input_is_refused():
     x = torch.zeros(64, 64, device="cuda")
     w = torch.zeros(64, 64, device="cuda")
