@@ -65,7 +65,7 @@ template <int ACT, bool SHORT> __device__ __forceinline__ float act_value_of(flo
     return z * (z > 0.f ? 1.f - q : q);
   }
   if constexpr (ACT == SGA_ACT_GELU_TANH)
-    return z * __builtin_amdgcn_rcpf(1.f + exp_f<SHORT>(-1.59576912160573072f * fmaf(0.044715f * z * z, z, z)));
+    return z * __builtin_amdgcn_rcpf(1.f + exp_f<SHORT>(-1.59576912f * fmaf(0.044715f * z * z, z, z)));
   if constexpr (ACT == SGA_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + exp_f<SHORT>(-z));
   return z;
 }
@@ -76,10 +76,10 @@ template <int ACT, bool SHORT> __device__ __forceinline__ float act_slope_of(flo
     return fmaf(z * 0.39894228040143268f, gauss, z > 0.f ? 1.f - q : q);
   }
   if constexpr (ACT == SGA_ACT_GELU_TANH) {
-    const float e = exp_f<SHORT>(-1.59576912160573072f * fmaf(0.044715f * z * z, z, z)), s = __builtin_amdgcn_rcpf(1.f + e);
+    const float e = exp_f<SHORT>(-1.59576912f * fmaf(0.044715f * z * z, z, z)), s = __builtin_amdgcn_rcpf(1.f + e);
     const float c = fminf(fmaxf(z, -16.f), 16.f);      // s (1 - s) is 0 beyond, and the polynomial must not be inf
     const float d = s * (s > 0.f ? e * s : 0.f);       // s (1 - s) without the difference
-    return fmaf(c * d, 1.59576912160573072f * fmaf(0.134145f * c, c, 1.f), s) + (z - z);
+    return fmaf(c * d, 1.59576912f * fmaf(0.134145f * c, c, 1.f), s) + (z - z);
   }
   if constexpr (ACT == SGA_ACT_SILU) {
     const float e = exp_f<SHORT>(-z), s = __builtin_amdgcn_rcpf(1.f + e);
