@@ -111,7 +111,7 @@ struct sga_handle {
   // The stream every step GRAPH is captured and launched on: the library's own, LOW priority (round 6).  Not for speed: on
   // ROCm 7.0.2 hipGraphLaunch on a NORMAL-priority stream crashes the host for some histories of streams that the process has
   // created and destroyed (scripts/r06/graph_stream_collision_repro.hip: 7 of 64 histories); on a launch stream of another
-  // priority class, whose hardware queues are a pool of their own, it never did.  The caller's stream is bridged in and out
+  // priority class it never did.  The caller's stream is bridged in and out
   // with one event pair per call (LaunchStream below); null: graphs run on the caller's stream (laboratory: SGA_LAUNCH_STREAM=caller)
   hipStream_t sG = nullptr;
   hipEvent_t ev_in = nullptr, ev_out = nullptr;
@@ -1765,8 +1765,8 @@ int sga_create(sga_handle** out, const sga_config* cfg, const sga_weights* w) {
     if (const char* hy = LAB_ENV("SGA_HYBRID")) h->side_hybrid = hy[0] == '1';
     {
       // LOW priority (numerically greatest): measured at cfg 2, the iteration takes 1773-1778 us on a low-priority launch stream,
-      // 1773-1775 on the caller's normal one and 1806-1816 on a HIGH-priority one (the hyper branch's kernels, on the graph's
-      // normal-priority internal stream, then lose every dispatch arbitration and become the critical path);
+      // 1773-1775 on the caller's normal one and 1806-1816 on a HIGH-priority one (the hyper branch
+      // then becomes the critical path);
       // profiles/r06_launch_stream_priority.txt.  Laboratory: SGA_LAUNCH_STREAM=caller (rounds 1-5: graphs on the caller's stream) | high
       const char* ls = LAB_ENV("SGA_LAUNCH_STREAM");
       const int want = (ls && strcmp(ls, "high") == 0) ? hi : (lo != 0 ? lo : hi);
