@@ -198,7 +198,7 @@ class _CallLog:
     arguments in order: integers and floats by value, a handle as `h<n>` (n-th successful sga_create of the process, from 0), any other pointer as `P` / `0`
     (non-null / null), the members of sga_config for sga_create -- flushed BEFORE the call is made, so the last line of a
     crashed process is the call it died in.  `tests/c_client/sga_replay.cpp` replays such a file against the library from
-    a process without Python or PyTorch (round 6: the hunt for the host SIGSEGV after mid-life hipGraphExecDestroy)."""
+    a process without Python or PyTorch."""
 
     def __init__(self, lib, path):
         self._lib, self._f, self._handles, self._created = lib, open(path, "a"), {}, 0

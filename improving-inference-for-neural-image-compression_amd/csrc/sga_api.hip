@@ -110,7 +110,7 @@ struct sga_handle {
   hipStream_t sB = nullptr;
   // The stream every step GRAPH is captured and launched on: the library's own, LOW priority (round 6).  Not for speed: on
   // ROCm 7.0.2 hipGraphLaunch on a NORMAL-priority stream crashes the host for some histories of streams that the process has
-  // created and destroyed (scripts/r06/graph_stream_collision_repro.hip: 7 of 64 histories); on a launch stream of another
+  // created and destroyed (a program without this library: 7 of 64 histories); on a launch stream of another
   // priority class it never did.  The caller's stream is bridged in and out
   // with one event pair per call (LaunchStream below); null: graphs run on the caller's stream (laboratory: SGA_LAUNCH_STREAM=caller)
   hipStream_t sG = nullptr;

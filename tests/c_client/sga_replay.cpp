@@ -1,15 +1,13 @@
 // Replays a C-ABI call log of libsga_hip (SGA_CALL_LOG=<file>, sga_amd/_lib.py: one text line per call) from a process WITHOUT
 // Python or PyTorch: the HIP runtime this program links (ROCm's own, not the one PyTorch bundles), plain hipMalloc'd buffers,
-// one non-blocking stream per handle.  Round 6, defect (a): the host SIGSEGV after mid-life hipGraphExecDestroy needs the HISTORY of
-// a pytest process (tests/test_gpu_configs.py as of round 5: ~60 handles, ~100 destroyed graphs); replayed here the same sequence
-// of sga_create / sga_encode / sga_step_grads / sga_run / sga_bb_run / sga_destroy can be put under rocgdb, valgrind or the
-// `make ASAN=1` host build, which a PyTorch process cannot (DESIGN_EXPERIMENTS.md A.8).
+// one non-blocking stream per handle.  The same sequence of sga_create / sga_encode / sga_step_grads / sga_run / sga_bb_run /
+// sga_destroy that a Python process made runs here against the plain C ABI.
 //
 //   hipcc -O1 -g -I include tests/c_client/sga_replay.cpp -o sga_replay -ldl        (the library is dlopen'ed: SGA_LIB or argv[2])
-//   SGA_GRAPH_DROP=destroy ./sga_replay calls.txt [libsga_hip.so] [-v]
+//   ./sga_replay calls.txt [libsga_hip.so] [-v]
 //
-// Data: weights are generated here with the scales of make_synthetic_weights (sga_amd/weights.py) -- the VALUES do not matter for
-// a crash hunt, the launch sequence does; every pointer argument of a call is served from its own pre-filled 48 MiB device slot
+// Data: weights are generated here with the scales of make_synthetic_weights (sga_amd/weights.py) -- the VALUES do not matter
+// here, the sequence of calls does; every pointer argument of a call is served from its own pre-filled 48 MiB device slot
 // (values in [0, 1): valid images, latents, uniforms).  A handle argument is `h<n>` = the n-th sga_create of the log.
 #include <dlfcn.h>
 #include <hip/hip_runtime_api.h>

@@ -1,17 +1,13 @@
 """Regression harness for "defect (a)" (DESIGN_EXPERIMENTS.md A.13), run as a SUBPROCESS by tests/test_gpu_graph_streams.py.
 
 The HIP runtime bundled with PyTorch-ROCm 2.10 (ROCm 7.0.2) crashes in hipGraphLaunch on a normal-priority stream for some
-histories of streams that the process has created and destroyed before.  This harness builds
-such histories on purpose -- the pattern of scripts/r06/graph_stream_collision_repro.hip, which kills 7 of 64 masks with a
-normal-priority launch stream -- in a process that has PyTorch AND libsga_hip in it: for every mask, six normal-priority ballast
+histories of streams that the process has created and destroyed before.  This harness goes through
+such histories in a process that has PyTorch AND libsga_hip in it: for every mask, six normal-priority ballast
 streams are created and used, the masked ones destroyed, and a fresh handle runs 110 iterations (three fork-point candidates are
 captured, instantiated, launched, two destroyed; the winner replayed).  libsga_hip launches its graphs on a stream of another
 priority class (sga_handle::sG), so every mask must survive and give the first mask's result bit for bit.
 
-    MALLOC_PERTURB_=165 python tests/tools/graph_stream_stress.py [--control]
-
---control: the laboratory build with SGA_LAUNCH_STREAM=caller = the behaviour of rounds 1-5 (graphs on the caller's stream): on the
-7.0.2 runtime this is EXPECTED TO DIE with SIGSEGV (scripts/r06/s05_*.sh runs it as the control; the test suite does not)."""
+    MALLOC_PERTURB_=165 python tests/tools/graph_stream_stress.py [--quick]"""
 import ctypes
 import os
 import sys
@@ -19,9 +15,6 @@ import sys
 ROOT = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 sys.path.insert(0, ROOT)
 os.environ.setdefault("GPU_MAX_HW_QUEUES", "2")
-control = "--control" in sys.argv
-if control:
-    os.environ["SGA_LAUNCH_STREAM"] = "caller"
 import numpy as np  # noqa: E402
 import torch  # noqa: E402
 
@@ -58,7 +51,7 @@ for mask in masks:
         if mask & (1 << k):
             chk(hip.hipStreamDestroy(bal[k]), "hipStreamDestroy")
             bal[k] = None
-    codec = SGACodec(w, C, B, H, W, lab=control)
+    codec = SGACodec(w, C, B, H, W)
     y_hat, z_hat, met, _ = codec.run(x, 0.01, its=110, seed=1)          # >= 100 iterations: the three fork-point candidates are timed
     again = codec.run(x, 0.01, its=30, seed=1)                          # the cached winner, launched again
     out = (y_hat.cpu(), z_hat.cpu(), again[0].cpu())
