@@ -67,11 +67,13 @@ template <> struct Mma<float, 16> {
   }
 };
 
-// 16 bytes per lane from buffer `srd` + voff into LDS at `lds` (wave-uniform) + lane * 16.  The wait is the caller's
-// (barrier_all): no register is written, so the compiler has nothing to track.
+// 16 bytes per lane from buffer `srd` + voff into LDS at `lds` (wave-uniform) + lane * 16.  The wait for the data is the caller's
+// (barrier_all): no register is written, so the compiler has nothing to track.  The waits in front of the fetch are made here, as the
+// compiler sees no fetch in this block: a scalar register that a vector instruction wrote (readfirstlane, or a spilled one read back)
+// may be used by a vector memory instruction 5 wait states later, and m0 1 later.
 __device__ __forceinline__ void dma16(uint32_t lds, uint32_t voff, i32x4 srd) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(srd) : "memory");      // m0 is reserved: the compiler sets it before any use of its own
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(srd) : "memory");      // m0 is reserved: the compiler sets it before any use of its own
 #endif
 }
 // everything this wave has in flight has landed, then all waves of the workgroup have got here

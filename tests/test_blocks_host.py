@@ -1,6 +1,10 @@
 """CPU tests of the token-block operators' argument checks (sga_amd.blocks and the C entry points): a call that cannot be carried
 out is refused before anything is launched."""
 import ctypes as C
+import os
+import re
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -157,3 +161,81 @@ def test_row_layouts():
         assert layout(t), t.shape
     for t in (base.t(), base.view(2, 3, 40)[:, :2], base.expand(3, 6, 40)):
         assert not layout(t), t.shape
+
+
+def scalar_registers(operand):
+    m = re.fullmatch(r"s(\d+)|s\[(\d+):(\d+)\]", operand.split(" ")[0])
+    if not m:
+        return ()
+    return (int(m.group(1)),) if m.group(1) else range(int(m.group(2)), int(m.group(3)) + 1)
+
+
+def short_waits(asm):
+    """-> (fetches into LDS, [(kernel, wait states, writer, fetch)] with fewer than 5 wait states between a vector instruction that
+    writes a scalar register and a vector memory instruction that uses it; the same for m0 and a fetch into LDS: fewer than 1).
+    Straight lines: every instruction is one wait state, s_nop n is n + 1."""
+    kernel, at, wrote, m0, fetches, short = None, 0, {}, -9, 0, []
+    for line in asm.splitlines():
+        m = re.match(r"[0-9a-f]+ <(\w+)>:", line)
+        if m:
+            kernel, wrote, m0 = m.group(1), {}, -9
+            continue
+        text = line.split("//")[0].strip()
+        if not line.startswith("\t") or not text:
+            continue
+        op, _, rest = text.partition(" ")
+        args = [a.strip() for a in rest.split(",")]
+        if op.startswith(("buffer_", "global_", "flat_", "scratch_")):
+            used = [r for a in args for r in scalar_registers(a)]
+            short += [(kernel, at - wrote[r][0] - 1, wrote[r][1], text) for r in used if r in wrote and at - wrote[r][0] - 1 < 5]
+            if text.endswith(" lds"):
+                fetches += 1
+                if at - m0 - 1 < 1:
+                    short.append((kernel, 0, "m0", text))
+        elif op.startswith("v_"):
+            carries = op.startswith(("v_cmp", "v_add_co", "v_sub_co", "v_subrev_co", "v_addc", "v_subb", "v_mad_u64", "v_mad_i64", "v_div_scale"))
+            for a in args[:2 if carries else 1]:
+                wrote.update((r, (at, text)) for r in scalar_registers(a))
+        elif op.startswith("s_"):
+            for r in scalar_registers(args[0]):
+                wrote.pop(r, None)
+            if args[0] == "m0":
+                m0 = at
+        at += int(args[0], 0) + 1 if op == "s_nop" else 1
+    return fetches, short
+
+
+def test_wait_states_are_counted():
+    """The counter itself, on lines with and without the waits."""
+    def lines(*ops):
+        return "0000 <k>:\n" + "\n".join("\t%s // x" % o for o in ops)
+    fetch = "buffer_load_dwordx4 v9, s[4:7], 0 offen lds"
+    start = ["v_readfirstlane_b32 s4, v1", "s_add_u32 s8, s8, s9", "s_mov_b32 m0, s10"]
+    assert short_waits(lines(*start, "s_nop 0", fetch))[1][0][1] == 3
+    assert short_waits(lines(*start, "s_nop 1", fetch))[1][0][1] == 4
+    assert short_waits(lines(*start, "s_nop 2", fetch)) == (1, [])
+    assert short_waits(lines("s_mov_b32 m0, s10", fetch))[1][0][2] == "m0"
+    assert short_waits(lines("v_readlane_b32 s4, v1, 3", "s_mov_b32 s4, s5", fetch.replace(" lds", ""))) == (0, [])      # written again by a scalar instruction
+    assert short_waits(lines("v_cmp_lt_u32_e64 s[6:7], v1, v2", fetch.replace(" lds", "")))[1]
+
+
+def test_fetches_into_lds_wait_for_their_scalar_registers(tmp_path):
+    """The matrix product's fetches are written by hand, where the compiler keeps no distances: every one of the built library has them."""
+    llvm = "/opt/rocm/lib/llvm/bin"
+    bundler, objdump = os.path.join(llvm, "clang-offload-bundler"), os.path.join(llvm, "llvm-objdump")
+    if not (os.path.exists(bundler) and os.path.exists(objdump) and shutil.which("objcopy")):
+        pytest.skip("no ROCm LLVM tools here")
+    fat = tmp_path / "fat.bin"
+    subprocess.run(["objcopy", "-O", "binary", "--only-section=.hip_fatbin", _lib.LIB_PATH, str(fat)], check=True)
+    data, total, short = fat.read_bytes(), 0, []
+    starts = [m.start() for m in re.finditer(re.escape(b"__CLANG_OFFLOAD_BUNDLE__"), data)] + [len(data)]
+    for b, e in zip(starts, starts[1:]):
+        one, co = tmp_path / "one.bin", tmp_path / "one.co"
+        one.write_bytes(data[b:e])
+        subprocess.run([bundler, "--unbundle", "--type=o", "--input=%s" % one, "--output=%s" % co, "--targets=hipv4-amdgcn-amd-amdhsa--gfx950"],
+                       check=True, capture_output=True)
+        asm = subprocess.run([objdump, "-d", str(co)], check=True, capture_output=True, text=True).stdout
+        n, s = short_waits(asm)
+        total += n
+        short += s
+    assert total > 500 and not short, (total, len(short), short[:4])
