@@ -294,7 +294,7 @@ __device__ __forceinline__ void epilogue1(const Epilogue& e, uint64_t seed, uint
 struct Operand { const void* p; int64_t ld; int strided; };
 struct Product {
   Operand x, w;
-  int64_t M, N, K;
+  int64_t M, N, K;               // at least 1 each
   int dtype;
   Epilogue e;
 };

@@ -90,6 +90,12 @@ __global__ __launch_bounds__(256) void token_sum_parts_kernel(const float* __res
   }
 }
 
+// g_weight of no rows, the sum of no terms: a product has at least one k (its tiles read the last one again for their ends)
+template <typename T>
+__global__ __launch_bounds__(256) void token_zero_kernel(T* __restrict__ out, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) out[i] = (T)0.f;
+}
+
 constexpr int kMaxFeatures = 1 << 20;
 constexpr int64_t kMaxRows = 0x7fffffff;
 
@@ -140,7 +146,7 @@ BwdPlan bwd_plan(const sga_linear& a, char* ws) {
     p.gx = {dz, {a.w, a.ld_w, 1}, a.rows, a.in_features, a.out_features, a.dtype, e};
     most = product_workspace(p.gx);
   }
-  if (a.g_w) {
+  if (a.g_w && a.rows > 0) {
     e.out = a.g_w;
     e.vec = a.in_features % 8 == 0 && aligned16(a.g_w);
     dz.strided = 1;
@@ -201,7 +207,13 @@ int linear_bwd(const sga_linear& a, char* ws, hipStream_t st) {
     const int s = launch_product(p.gx, ws + p.prod_off, st);
     if (s != SGA_OK) return s;
   }
-  return a.g_w ? launch_product(p.gw, ws + p.prod_off, st) : SGA_OK;
+  if (a.g_w && a.rows > 0) return launch_product(p.gw, ws + p.prod_off, st);
+  if (a.g_w) {
+    const int64_t n = (int64_t)a.out_features * a.in_features, blocks = ceil_div(n, 256);
+    hipLaunchKernelGGL((token_zero_kernel<T>), dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, st, (T*)a.g_w, n);
+    LAUNCHED();
+  }
+  return SGA_OK;
 }
 
 }  // namespace

@@ -493,6 +493,25 @@ def test_no_rows():
     assert b.dropout(x, 0.5, 1).shape == (0, 24)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("inn,out", [(5, 12), (12, 33), (33, 5), (1, 1), (24, 8), (130, 257)])
+@pytest.mark.parametrize("act,p", [("none", 0.0), ("silu", 0.0), ("none", 0.5), ("relu", 0.5)])
+def test_no_rows_of_any_width(act, p, inn, out, dtype):
+    """Weight gradients of no rows are zeros at widths that fill no 16-byte piece too, and the call writes nothing else: empty tensors
+    without memory, and empty cuts of a wider buffer (whose rows start anywhere)."""
+    b, t = blocks(), TYPES[dtype]
+    w = torch.ones(out, inn + 3, dtype=t, device="cuda")[:, 1:1 + inn]
+    room = torch.full((4, max(inn, out) + 3), 7.0, dtype=t, device="cuda")
+    drop = (p, SEED, OFFSET) if p else None
+    for x, g in ((torch.empty(0, inn, dtype=t, device="cuda"), torch.empty(0, out, dtype=t, device="cuda")), (room[2:2, 1:1 + inn], room[2:2, 1:1 + out])):
+        pre = torch.empty(0, out, dtype=t, device="cuda")
+        g_x, g_w, g_b = b.linear_grad(g, x, w, pre=pre, act=act, dropout=drop)
+        assert g_x.shape == (0, inn) and g_w.shape == (out, inn) and g_w.dtype == t
+        assert torch.equal(g_w, torch.zeros_like(g_w)) and torch.equal(g_b, torch.zeros_like(g_b))
+        assert torch.equal(b.linear_grad(g, x, w, pre=pre, act=act, dropout=drop, want=(False, True, False))[1], g_w)
+    assert (room == 7).all()
+
+
 def block64(x, nw, nb, w1, b1, w2, b2, p):
     C = x.shape[-1]
     d = x - x.mean(1, keepdim=True)
