@@ -15,7 +15,8 @@ A token is a row: the last dimension holds the features, all others are tokens -
 float32, bfloat16 or float16 tensors of one device; sums and statistics in float32, one rounding on store.  The last dimension has
 stride 1, the dimensions before it one common stride (a slice of a wider buffer, an expanded row); anything else is
 refused, not copied.  Calls run on the current stream of the tensors' device and take their outputs and workspace from torch's
-allocator, so they may be captured into a graph; results carry no autograd history.  `dropout` is (p, seed, offset), or (p, state) with `state` an int64 tensor
+allocator, so they may be captured into a graph; results carry no autograd history, but a tensor written through `out` counts
+as changed in place: autograd refuses a backward pass that needs what it held, and an `out` that requires a gradient is refused.  `dropout` is (p, seed, offset), or (p, state) with `state` an int64 tensor
 {seed, offset} on the device that is read when the kernel runs (a captured graph draws new numbers when it changes).
 There is no CPU path.
 """
@@ -191,13 +192,16 @@ def linear(x, weight, bias=None, act="none", residual=None, dropout=None, want_p
         _, _, ld_res = _rows(residual, "residual", dt, dev, n)
         _same(residual, shape, "residual")
         p_res = residual.data_ptr()
-    if out is None:
+    given = out is not None
+    if not given:
         out = x.new_empty(shape)
     else:
         _, _, ld_out = _rows(out, "out", dt, dev, n)
         _same(out, shape, "out")
         if ld_out == 0 and rows > 1:
             raise ValueError("out: its rows overlap")
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError("out requires a gradient, which the call would not record")
         _apart(out, rows, n, ld_out, x, "x", rows, k, ld_x)
         _apart(out, rows, n, ld_out, weight, "weight", n, k, ld_w)
         _apart(out, rows, n, ld_out, bias, "bias", 1, n, n)
@@ -209,6 +213,8 @@ def linear(x, weight, bias=None, act="none", residual=None, dropout=None, want_p
     a = _LINEAR(rows, k, n, _DTYPES[dt], _act(act), x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _vector(bias, "bias", n, (dt,), dev), p_res, ld_res,
                 out.data_ptr(), ld_out, p_pre, 0, 0, 0, 0, 0, *_drop(dropout, dev))
     _call_with_workspace("sga_op_linear_fwd", a, dev, 0)
+    if given:
+        torch.autograd.graph.increment_version(out)
     return (out, pre) if want_pre else out
 
 

@@ -706,3 +706,25 @@ def test_linear_with_an_output_over_its_input_is_refused():
     both = torch.randn(64, 128, device="cuda")                   # columns side by side in one buffer
     want = blocks().linear(both[:, :64].contiguous(), w)
     assert torch.equal(blocks().linear(both[:, :64], w, out=both[:, 64:]), want)
+
+
+def test_linear_with_an_output_is_a_change_in_place():
+    """Autograd notices that a tensor it saved was written to, through any view of it; an `out` that requires a gradient is refused."""
+    x, w = torch.randn(4, 64, device="cuda"), torch.randn(64, 64, device="cuda")
+    y = torch.randn(4, 64, device="cuda", requires_grad=True).exp()      # its backward pass needs y
+    for out in (y.detach(), y.detach()[:, 0:64]):
+        before = y._version
+        assert blocks().linear(x, w, out=out) is out and y._version == before + 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    leaf = torch.zeros(4, 64, device="cuda", requires_grad=True)
+    for out in (y, leaf):
+        before = out.detach().clone()
+        with pytest.raises(ValueError, match="requires a gradient"):
+            blocks().linear(x, w, out=out)
+        assert torch.equal(out.detach(), before)
+    with torch.no_grad():
+        blocks().linear(x, w, out=leaf)
+    assert torch.equal(leaf.detach(), blocks().linear(x, w))
+    with torch.inference_mode():
+        assert torch.equal(blocks().linear(x, w, out=torch.empty(4, 64, device="cuda")), leaf.detach())
