@@ -98,6 +98,18 @@ def _vector(t, what, n, dtypes, device):
     return t.data_ptr()
 
 
+def _param_type(weight, bias, dt):
+    """The type of a norm's parameters: weight's (bias's without a weight), which is x's type `dt` or float32; `dt` where there are none."""
+    t, what = (weight, "weight") if weight is not None else (bias, "bias")
+    if t is None:
+        return dt
+    if not isinstance(t, _Tensor):
+        raise TypeError("%s: a tensor is expected, got %s" % (what, type(t).__name__))
+    if t.dtype != dt and t.dtype != torch.float32:
+        raise TypeError("%s: %s or torch.float32 is expected, got %s" % (what, dt, t.dtype))
+    return t.dtype
+
+
 def _like(x):
     """A tensor for a result of x's shape and type (rows without gaps)."""
     return _empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
@@ -187,6 +199,7 @@ def linear(x, weight, bias=None, act="none", residual=None, dropout=None, want_p
     if weight.dim() != 2:
         raise ValueError("weight: [out_features, in_features] is expected, got shape %s" % (tuple(weight.shape),))
     shape = x.shape[:-1] + (n,)
+    p_bias = _vector(bias, "bias", n, (dt,), dev)
     ld_res, ld_out, p_res, p_pre, pre = n, n, 0, 0, None
     if residual is not None:
         _, _, ld_res = _rows(residual, "residual", dt, dev, n)
@@ -210,7 +223,7 @@ def linear(x, weight, bias=None, act="none", residual=None, dropout=None, want_p
     if want_pre:
         pre = x.new_empty(shape)
         p_pre = pre.data_ptr()
-    a = _LINEAR(rows, k, n, _DTYPES[dt], _act(act), x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _vector(bias, "bias", n, (dt,), dev), p_res, ld_res,
+    a = _LINEAR(rows, k, n, _DTYPES[dt], _act(act), x.data_ptr(), ld_x, weight.data_ptr(), ld_w, p_bias, p_res, ld_res,
                 out.data_ptr(), ld_out, p_pre, 0, 0, 0, 0, 0, *_drop(dropout, dev))
     _call_with_workspace("sga_op_linear_fwd", a, dev, 0)
     if given:
@@ -250,8 +263,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, want_stats=False):
     want_stats: -> (y, mean, rstd), the last two float32 of x's leading shape, which `layer_norm_grad` needs."""
     rows, n, ld = _rows(x, "x")
     dt, dev = x.dtype, x.device
-    pt = weight.dtype if weight is not None else bias.dtype if bias is not None else dt
-    w, b = _vector(weight, "weight", n, (dt, torch.float32), dev), _vector(bias, "bias", n, (pt,), dev)
+    pt = _param_type(weight, bias, dt)
+    w, b = _vector(weight, "weight", n, (pt,), dev), _vector(bias, "bias", n, (pt,), dev)
     if not eps >= 0.0:
         raise ValueError("eps: a number >= 0 is expected, got %r" % (eps,))
     y = _like(x)

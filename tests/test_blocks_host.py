@@ -239,3 +239,20 @@ def test_fetches_into_lds_wait_for_their_scalar_registers(tmp_path):
         total += n
         short += s
     assert total > 500 and not short, (total, len(short), short[:4])
+
+
+def test_parameter_types_of_a_norm():
+    """weight and bias have x's type or float32, whichever of them is given; anything else is a TypeError."""
+    for x in (torch.float32, torch.bfloat16, torch.float16):
+        assert blocks._param_type(None, None, x) == x
+        for t in (x, torch.float32):
+            p = torch.ones(4, dtype=t)
+            assert blocks._param_type(p, None, x) == blocks._param_type(None, p, x) == blocks._param_type(p, p, x) == t
+        for t in {torch.float64, torch.int32, torch.bool, torch.float16, torch.bfloat16} - {x}:
+            p = torch.ones(4).to(t)
+            for args in ((p, None), (None, p), (p, torch.ones(4))):
+                with pytest.raises(TypeError):
+                    blocks._param_type(*args, x)
+        for args in (([1.0] * 4, None), (None, [1.0] * 4), (None, 1.0)):
+            with pytest.raises(TypeError):
+                blocks._param_type(*args, x)

@@ -728,3 +728,14 @@ def test_linear_with_an_output_is_a_change_in_place():
     assert torch.equal(leaf.detach(), blocks().linear(x, w))
     with torch.inference_mode():
         assert torch.equal(blocks().linear(x, w, out=torch.empty(4, 64, device="cuda")), leaf.detach())
+
+
+def test_wrong_parameter_types_are_refused():
+    x, w, out = torch.ones(4, 8, device="cuda"), torch.ones(8, 8, device="cuda"), torch.zeros(4, 8, device="cuda")
+    for bad in (torch.ones(8, device="cuda", dtype=torch.float64), torch.ones(8, device="cuda", dtype=torch.int32), [1.0] * 8, torch.ones(8)):
+        error = ValueError if isinstance(bad, torch.Tensor) and bad.dtype == torch.float32 else TypeError      # right type, wrong device
+        for call in (lambda: blocks().layer_norm(x, None, bad), lambda: blocks().layer_norm(x, bad), lambda: blocks().layer_norm(x, x[0], bad),
+                     lambda: blocks().linear(x, w, bad), lambda: blocks().linear(x, w, bad, out=out)):
+            with pytest.raises(error):
+                call()
+    assert float(out.abs().max()) == 0.0
