@@ -97,7 +97,7 @@ __global__ __launch_bounds__(256) void token_zero_kernel(T* __restrict__ out, in
 }
 
 constexpr int kMaxFeatures = 1 << 20;
-constexpr int64_t kMaxRows = 0x7fffffff;
+constexpr int64_t kMaxRows = 0x7fffff00;      // as many as 256-row tiles of 512 lanes fit into a launch of 2^32 lanes
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 

@@ -613,7 +613,7 @@ __global__ __launch_bounds__(256) void token_pack_kernel(const U* __restrict__ s
 // How a product is run
 struct Plan {
   int few;                   // 16-row blocks of token_few_kernel, 0: tiles
-  int tile;                  // index into the tile table
+  int tile;                  // index into the tile table; -1: too many tiles for a launch
   int nsplit;
   bool pack_x, pack_w;
   int64_t ldp_x, ldp_w;      // elements, packed
@@ -631,7 +631,12 @@ bool needs_pack(const Operand& o, int64_t rows, int E) {
 // The tiles and what they cost, measured over 20 shapes from 32 x 4096 x 4096 to 8192 x 16384 x 4096 (128 to 8192 workgroups, K splits 1
 // to 8; the plan found is within 6 % of the fastest there): ns of a K step of a workgroup with 1 and with 2 of them on its CU (as
 // many as the LDS holds), 16- and 32-bit types, and of the rest of a tile's life.
-struct Tile { int m, n, per_cu; double step[2][2], once; };
+struct Tile {
+  int m, n, per_cu;
+  double step[2][2], once;
+  constexpr int lanes() const { return m * n > 8192 ? 512 : 256; }      // of a workgroup (run_tile_of)
+};
+constexpr int64_t kMaxLanes = 0xffffffff;      // of a launch: the grid is counted in lanes, in 32 bits, and one past that starts over at 0
 constexpr int kTiles = 5;
 const Tile kTile[kTiles] = {{256, 256, 1, {{1600, 0}, {7350, 0}}, 9000},
                             {256, 128, 1, {{930, 0}, {3800, 0}}, 5000},
@@ -659,6 +664,7 @@ Plan make_plan(const Product& p) {
   // element by element, 4 us more at the end of a tile, which the join's many small workgroups do not feel
   const bool off = (((uint64_t)(uintptr_t)p.x.p | (uint64_t)(p.x.ld * E) | (uint64_t)(uintptr_t)p.w.p | (uint64_t)(p.w.ld * E)) & 15) != 0;
   double best = 1e300;
+  o.tile = -1;
   o.nsplit = 1;
   for (int t = 0; t < kTiles; ++t) {
     if (kTile[t].m == 96 && p.x.strided) continue;      // the keys of a k row need a power of two
@@ -666,6 +672,7 @@ Plan make_plan(const Product& p) {
     const Tile& c = kTile[t];
     const double* step = c.step[E == 4];
     for (int s = 1; s == 1 || (s <= 16 && s <= nk); ++s) {
+      if (tiles * s * c.lanes() > kMaxLanes) continue;
       const int64_t at_once = (int64_t)kCUs * c.per_cu, rest = tiles * s % at_once;
       const double steps = (double)ceil_div(nk, s);
       double cost = (double)(tiles * s / at_once) * (steps * step[c.per_cu - 1] + c.once);
@@ -682,6 +689,7 @@ Plan make_plan(const Product& p) {
 template <typename T, int MF, int TM, int TN, int WM, int WN, int NS, bool XS, bool WS>
 int run_tile(const TileArgs& a, hipStream_t st) {
   constexpr int BM = WM * TM * MF, BN = WN * TN * MF, MAIN = NS * (BM + BN) * 128, EPI = WM * WN * MF * (TN * MF + 4) * 4;
+  static_assert(WM * WN * 64 == Tile{BM, BN}.lanes(), "the plan counts on it");
   constexpr int LDS = MAIN > EPI ? MAIN : EPI;
   const void* f = reinterpret_cast<const void*>(&token_tile_kernel<T, MF, TM, TN, WM, WN, NS, XS, WS>);
   if (LDS > 65536 && hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return SGA_ERR_HIP;
@@ -729,6 +737,7 @@ int run_few(const Product& p, hipStream_t st) {
 template <typename T>
 int run(const Product& p, char* ws, hipStream_t st) {
   const Plan o = make_plan(p);
+  if (o.tile < 0) return SGA_ERR_UNSUPPORTED;
   if (o.few) return o.few == 1 ? run_few<T, 1>(p, st) : o.few == 2 ? run_few<T, 2>(p, st) : run_few<T, 4>(p, st);
   TileArgs a = {};
   typedef typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type U;
@@ -756,7 +765,6 @@ int run(const Product& p, char* ws, hipStream_t st) {
   a.part = o.nsplit > 1 ? (float*)(ws + o.part_off) : nullptr;
   a.ld_part = o.ld_part;
   a.e = p.e;
-  if ((int64_t)a.ntm * a.ntn * a.nsplit > 0x7fffffff) return SGA_ERR_UNSUPPORTED;
   s = run_order<T>(o.tile, p.x.strided, p.w.strided, a, st);
   if (s != SGA_OK || o.nsplit == 1) return s;
   if (p.e.vec)

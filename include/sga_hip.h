@@ -366,7 +366,7 @@ typedef struct sga_dropout {
  * z [rows, out_features], contiguous.  Backward: dz = D_p(g_out) act'(pre) (of act = RELU: 0 at 0), rounded to `dtype` as the
  * operand of g_x [rows, in_features] = dz w and g_w [out_features, in_features] = dz^T x; g_bias [out_features] = sum of dz over
  * rows.  g_x, g_w, g_bias are contiguous, any of them NULL = not wanted; the gradient of `residual` is g_out itself.
- * residual may be out itself (same ld).  Limits: in_features, out_features <= 2^20, rows < 2^31. */
+ * residual may be out itself (same ld).  Limits: in_features, out_features <= 2^20, rows <= 2^31 - 256. */
 typedef struct sga_linear {
   int64_t rows;
   int32_t in_features, out_features, dtype, act;

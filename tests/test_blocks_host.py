@@ -256,3 +256,17 @@ def test_parameter_types_of_a_norm():
         for args in (([1.0] * 4, None), (None, [1.0] * 4), (None, 1.0)):
             with pytest.raises(TypeError):
                 blocks._param_type(*args, x)
+
+
+def test_linear_row_limit():
+    """More rows than the tiles of one launch can cover are refused, up to there they are not."""
+    lib = _lib.load_library()
+    n = C.c_int64(0)
+    most = (1 << 31) - 256
+    for backward in (0, 1):
+        for features in (1, 8):
+            a = dict(in_features=features, out_features=features)
+            assert lib.sga_op_linear_workspace(C.byref(linear(rows=most, **a)), backward, C.byref(n)) == 0
+            assert lib.sga_op_linear_workspace(C.byref(linear(rows=most + 1, **a)), backward, C.byref(n)) == UNSUPPORTED
+    assert lib.sga_op_linear_fwd(C.byref(linear(rows=most + 1)), None, 0, None) == UNSUPPORTED
+    assert lib.sga_op_linear_bwd(C.byref(linear(rows=most + 1)), P, 1 << 62, None) == UNSUPPORTED

@@ -739,3 +739,21 @@ def test_wrong_parameter_types_are_refused():
             with pytest.raises(error):
                 call()
     assert float(out.abs().max()) == 0.0
+
+
+def test_linear_of_the_most_rows():
+    """A launch counts its lanes in 32 bits: with as many rows as are allowed, every one of them is written."""
+    rows = 2 ** 31 - 256
+    x = torch.arange(256, device="cuda").to(torch.bfloat16).repeat(rows // 256).view(rows, 1)
+    w = torch.full((1, 1), 2.0, dtype=torch.bfloat16, device="cuda")
+    y = blocks().linear(x, w)
+    for first in range(0, rows, 2 ** 28):
+        part = slice(first, first + 2 ** 28)
+        assert torch.equal(y[part], x[part] * 2), first
+    del y
+    g_x, _, _ = blocks().linear_grad(x, x, w, want=(True, False, False))
+    for first in range(0, rows, 2 ** 28):
+        part = slice(first, first + 2 ** 28)
+        assert torch.equal(g_x[part], x[part] * 2), first
+    with pytest.raises(RuntimeError, match="UNSUPPORTED"):
+        blocks().linear(torch.zeros(1, 1, dtype=torch.bfloat16, device="cuda").expand(rows + 1, 1), w)
