@@ -29,8 +29,8 @@ template <bool SHORT> __device__ __forceinline__ float exp_f(float x) {
 }
 
 // Phi(-|z|) = erfc(|z| / sqrt 2) / 2 = g(|z|) e^(-z^2 / 2) with g smooth and slowly varying: g as a polynomial in t = 1 / (1 + 0.3 |z|),
-// fitted on 0 <= |z| <= 14 for the least maximum of the relative error (beyond, the exponential is 0): degree 8 is off by 5.8e-8 in
-// exact arithmetic, 5e-7 with float32 steps; degree 6, for SHORT results, by 1.9e-6.  Relative accuracy in the tail is what
+// fitted on 0 <= |z| <= 14 for the least maximum of the relative error (beyond, the exponential is 0): degree 8, with its constants as
+// float32 holds them, is off by 1.1e-7 in exact arithmetic, 4e-7 with float32 steps; degree 6, for SHORT results, by 1.9e-6 and 2.2e-6.  Relative accuracy in the tail is what
 // 1 + erf(z) cannot give, and the backward pass shares the exponential: about 25 (SHORT: 18) instructions where the
 // library's erf and exp take about 60.
 template <bool SHORT> __device__ __forceinline__ float normal_tail(float z, float gauss) {

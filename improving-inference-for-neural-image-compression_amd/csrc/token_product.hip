@@ -419,8 +419,9 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void token_tile_kernel(const TileA
 }
 
 // ---- few rows of X (tokens of as many sequences): the weight's rows are read once, straight into fragments ------------------
-// A workgroup of 8 waves owns 16 columns n, or 8 where 16 would leave CUs idle (1 x 8192 x 2048 bf16: 9.3 us, with 16 columns 12.0; 16 rows 14.5
-// against 16.9).  The waves share out K in pieces of 128 bytes per row of w, so that a wave reads whole
+// A workgroup of 8 waves owns 16 columns n, or 8 as long as that is one round of workgroups over the CUs, up to N = 2048 (1 x 8192 x 2048
+// bf16: 9.3 us, with 16 columns 12.0; 16 rows 14.5 against 16.9).  Past it a second round costs more than the CUs that 16 columns leave
+// idle: N = 2056, 16 columns 12.5 us, 8 columns 16.1; 16 rows 19.6 against 26.1; N = 4088 17.3 against 20.2.  The waves share out K in pieces of 128 bytes per row of w, so that a wave reads whole
 // lines; MFMA rows = the 16 columns, MFMA columns = 16 rows of X (MB of them).  Any order of k inside a piece serves, as both
 // operands take the same: lane (r, q) takes bytes q * 16 .. of each 64.  The waves' sums meet in LDS.
 // Bound by the weight's bytes and, when small, by latency: one row of 4096 x 4096 bf16 (34 MB) 8.2 us = 4.1 TB/s, 12 rows of
@@ -648,7 +649,7 @@ constexpr int kCUs = 256;
 Plan make_plan(const Product& p) {
   const int E = (int)dtype_bytes(p.dtype), V = 16 / E;
   Plan o = {};
-  // token_few_kernel reads X again for every 16 columns, the tiles in whole tile rows: at 16 rows and 4096 x 4096 weights (bf16) 11.0 us
+  // token_few_kernel reads X again for every 8 or 16 columns, the tiles in whole tile rows: at 16 rows and 4096 x 4096 weights (bf16) 11.0 us
   // against 14.7, at 32 rows 13.9 against 12.7; up to 64 rows where there is little to read at all (1024 x 1024: 7.0 against 8.3) and
   // rows are short (48 rows, 160 x 7376, odd rows: 66 us, as its 10 workgroups go along K alone; the tiles, which split K, 16)
   if (!p.x.strided && !p.w.strided && (p.M <= 16 || (p.M <= 64 && p.K * E <= 4096 && p.M * p.N * p.K <= 1 << 26))) {

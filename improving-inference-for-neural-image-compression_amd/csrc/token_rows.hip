@@ -305,7 +305,8 @@ __device__ __forceinline__ float block_sum(float v, float* sh) {
 
 // ---- rows too long for registers: read again for each pass (the second and third time from L2) ------------------------------
 // For widths past 16384, kept simple: bound by HBM and L2, a workgroup of 256 per row, single elements a lane, so any
-// alignment.  4096 x 20000 bf16 (328 MB) 184 us = 1.8 TB/s; its gradients (492 MB) 311 us.
+// alignment.  4096 x 20000 bf16 (328 MB) 250 us = 1.3 TB/s with inputs that change (184 with one that stays in the last-level cache); its
+// gradients with g_add (656 MB) 516 us.
 template <typename T, typename P>
 __global__ __launch_bounds__(256) void layer_norm_fwd_long_kernel(const T* __restrict__ x, int64_t ld_x, const P* __restrict__ w,
                                                                   const P* __restrict__ b, T* __restrict__ y, float* __restrict__ mean,

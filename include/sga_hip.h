@@ -387,7 +387,7 @@ int sga_op_linear_fwd(const sga_linear* a, void* workspace, int64_t workspace_by
 int sga_op_linear_bwd(const sga_linear* a, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* y = (x - mean) rstd w + b per row of x [rows, cols], rstd = 1 / sqrt(var + eps), var the mean of (x - mean)^2 (two passes over
- * the row on chip); w, b [cols] of type param_dtype (dtype or F32), NULL = 1 and 0.  mean, rstd [rows] float32: written by the
+ * the row); w, b [cols] of type param_dtype (dtype or F32), NULL = 1 and 0.  mean, rstd [rows] float32: written by the
  * forward pass (NULL = not wanted), read by the backward pass:  g = g_y w, h = (x - mean) rstd,
  * g_x = g_add + rstd (g - mean(g) - h mean(g h)), g_w = sum of g_y h, g_b = sum of g_y over rows.  g_add [rows, cols]
  * (optional): the gradient that reaches x past the norm.  y, g_x, g_w, g_b contiguous, any of g_x, g_w, g_b NULL = not
